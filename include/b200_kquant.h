@@ -55,7 +55,8 @@ enum {
     B200_TYPE_Q4_K = 12, /* 256 elements / 144 bytes */
     B200_TYPE_Q6_K = 14, /* 256 elements / 210 bytes */
     B200_TYPE_I32 = 26,
-    B200_TYPE_BF16 = 30  /* weights of stages created with b200_stage_create_layers */
+    B200_TYPE_BF16 = 30, /* weights of stages created with b200_stage_create_layers */
+    B200_TYPE_F8_E4M3 = 100 /* pages of b200_kv_pages_append only (no ggml id) */
 };
 
 /* ---- ops understood by graph_compute (the subset on the hot path) -------------------------- */
@@ -273,6 +274,51 @@ B200_API b200_status b200_attention_kv(const float *q, const void *k_cache, cons
                                        uint32_t k_type, uint32_t v_type, int64_t T, int64_t pos0,
                                        int64_t n_head, int64_t n_kv, int64_t hd, float *out,
                                        void *scratch, size_t scratch_bytes, void *stream);
+/* A key / value cache in pages, for sequences of unlike length that share one pool (the counterpart of the
+ * contiguous caches above; the reference leaves this to its server).  Pools k and v: [n_pages][n_kv][page_size]
+ * [head_dim], page_stride elements from one page to the next (0: dense), of type f16, or e4m3 with one scale per
+ * aligned block of 16 positions and head, k_scale and v_scale [n_pages][n_kv][page_size / 16].  A scale is a power
+ * of two from 2^-15 to 2^7, so code times scale is an f16 number.  head_dim 64 or 128, page_size a multiple of 16.
+ * A batch: row r of its `rows` rows belongs to the sequence s with row_start[s] <= r < row_start[s + 1] (ascending,
+ * n_seq + 1 entries; rows no sequence owns are left alone) and stands at position pos0[s] + r - row_start[s];
+ * table[s][i] is the page of positions i page_size .. of sequence s, table_len entries that are table_stride apart.
+ * row_start, pos0 and table are device memory, read by the kernels: a captured graph follows what they hold at its replay.
+ * A table entry outside 0 .. n_pages - 1, a position past the table and every position of a sequence with
+ * pos0 < 0 are not there: neither stored nor seen.                                              */
+typedef struct b200_kv_pages {
+    void *k, *v;
+    float *k_scale, *v_scale; /* NULL for f16 */
+    int64_t n_pages, page_stride;
+    uint32_t type;
+    int32_t page_size, n_kv, head_dim;
+} b200_kv_pages;
+typedef struct b200_page_batch {
+    const int32_t *row_start, *pos0, *table;
+    int64_t rows;
+    int32_t n_seq, table_len, table_stride;
+} b200_page_batch;
+/* Writes the rows' keys, rotated at their positions (theta 0: as they come; neox as in b200_rope; angles in 64
+ * bits), and values into their pages.  k, v: [rows][n_kv][head_dim] of type f32, f16 or bf16, rows k_stride and
+ * v_stride elements apart, 16-byte aligned.  Rows of a block of e4m3 positions go in under the larger of its scale
+ * (where it holds earlier positions, whose codes are rescaled) and what the largest new value asks for.  A value beyond the
+ * page type's range becomes the largest one; a NaN in v becomes 0 there and NaN at its place in the token's k, so
+ * that exactly the queries that see the token give NaN.  Two sequences of one call must not write the same page.  */
+B200_API b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type,
+                                          const void *k, int64_t k_stride, const void *v, int64_t v_stride, float theta,
+                                          int32_t neox, void *stream);
+/* Causal attention of the batch's rows over their sequences' pages: head h of a row at position p sees positions
+ * p - window + 1 .. p (window 0: from 0 on) that are there, of KV head h / (n_head / n_kv); a row that sees none is 0.
+ * q, out: [rows][n_head][head_dim] of type f32, f16 or bf16, q_stride and out_stride elements between rows, 16-byte aligned;
+ * the queries are rotated on the way in (theta 0: as they come).  scale 0: 1 / sqrt(head_dim).  max_rows: the most rows of a
+ * sequence as far as the caller knows; it picks the kernels, any value is right.  f32: queries and probabilities enter
+ * the products in two f16 parts, results are good to 32 bits; f16, bf16: probabilities in one f16 part.
+ * scratch: b200_attention_pages_scratch_bytes of device memory, 16-byte aligned, of any content; calls that share it must be
+ * ordered on one stream.                                                                        */
+B200_API size_t b200_attention_pages_scratch_bytes(const b200_kv_pages *cache, int32_t n_head, int32_t max_rows);
+B200_API b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type,
+                                          const void *q, int64_t q_stride, int32_t n_head, int32_t max_rows, float theta,
+                                          int32_t neox, int32_t window, float scale, void *out, int64_t out_stride,
+                                          void *scratch, size_t scratch_bytes, void *stream);
 B200_API b200_status b200_get_rows(uint32_t type, const void *W, const int32_t *ids, int64_t T,
                                    int64_t K, float *y, void *stream);
 B200_API b200_status b200_argmax(const float *x, int64_t T, int64_t n, int32_t *idx, void *stream);

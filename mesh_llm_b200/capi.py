@@ -12,6 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.environ.get("B200_KQ_LIB") or os.path.join(_HERE, "libb200kq.so")
 
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_I32, TYPE_BF16 = 0, 1, 2, 8, 12, 14, 26, 30
+TYPE_F8_E4M3 = 100  # cache pages
 
 OK = 0
 STATUS_NAMES = {0: "OK", -1: "INVALID", -2: "ALLOC", -3: "CUDA", -4: "UNSUPPORTED", -5: "BOUNDS",
@@ -77,6 +78,17 @@ class StackConfig(C.Structure):
         ("precision", C.c_int32), ("embd_scale", C.c_float), ("norm_offset", C.c_float),
         ("norm_place", C.c_int32), ("side_dim", C.c_int32), ("logit_softcap", C.c_float),
     ]
+
+
+class KvPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_int64), ("page_stride", C.c_int64), ("type", C.c_uint32),
+                ("page_size", C.c_int32), ("n_kv", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class PageBatch(C.Structure):
+    _fields_ = [("row_start", C.c_void_p), ("pos0", C.c_void_p), ("table", C.c_void_p), ("rows", C.c_int64),
+                ("n_seq", C.c_int32), ("table_len", C.c_int32), ("table_stride", C.c_int32)]
 
 
 class GgufMeta(C.Structure):
@@ -167,6 +179,10 @@ SIGNATURES = {
     "b200_kv_types_for_model_bytes": (None, [u64, C.POINTER(u32), C.POINTER(u32)]),
     "b200_kv_store": (i32, [vp, vp, vp, i64, i64, i64, C.c_float, i32, u32, u32, vp, vp, vp]),
     "b200_attention_kv": (i32, [vp, vp, vp, u32, u32, i64, i64, i64, i64, i64, vp, vp, sz, vp]),
+    "b200_kv_pages_append": (i32, [C.POINTER(KvPages), C.POINTER(PageBatch), u32, vp, i64, vp, i64, C.c_float, i32, vp]),
+    "b200_attention_pages_scratch_bytes": (sz, [C.POINTER(KvPages), i32, i32]),
+    "b200_attention_pages": (i32, [C.POINTER(KvPages), C.POINTER(PageBatch), u32, vp, i64, i32, i32, C.c_float, i32, i32,
+                                   C.c_float, vp, i64, vp, sz, vp]),
     "b200_get_rows": (i32, [u32, vp, vp, i64, i64, vp, vp]),
     "b200_argmax": (i32, [vp, i64, i64, vp, vp]),
     "b200_mul_mat_id_scratch_bytes": (sz, [i64, i64, i64, i64]),

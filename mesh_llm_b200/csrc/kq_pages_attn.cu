@@ -1,0 +1,550 @@
+// Attention of a few new rows per sequence over paged keys and values (b200_attention_pages): decode steps and drafts.
+//
+// A warp takes 16 positions (f16) or 32 (e4m3) of an item at a time straight from the pages into registers, as the fragments
+// of mma.m16n8k16: nothing goes through shared memory.  That works because the order of a product's inner index is free: a thread
+// reads 16 bytes of a key, which are the dimensions that its lane holds in consecutive steps of Q K^T, and Q is laid out to match; of the
+// values it reads 16 bytes of four keys and pairs them up by byte permutes into the rows of V^T.  e4m3 codes become f16 in
+// registers (K's scale goes onto the score, V's onto the value, both exact powers of two).  Scores are Q K^T with the item's rows as
+// the 16 rows of the tile; the probabilities are then already the B operand of O^T = V^T P^T.  Softmax in base 2, statistics in 32 bits.
+// A query row enters divided by the power of two that brings its largest element to [1, 2), so f16 neither overflows nor loses small
+// rows; f32 rows go in as two f16 parts (22 bits), and so do their probabilities.
+//
+// Bound by HBM: a position costs 2 hd codes per KV head and is read once.  The units of all items are shared out evenly
+// (kq_pages_sched.cuh), the four warps of a CTA take neighbouring positions and join their rows through shared memory at an item's end.
+#include "kq_pages_sched.cuh"
+
+#include <math.h>
+
+namespace {
+
+constexpr int NT = 128, NW = NT / 32;
+constexpr int MAX_CTAS_PER_SM = 4;
+
+__device__ __forceinline__ uint4 ld16(const uint8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 ld8(const uint8_t *p) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t h2_low(float a, float b, uint32_t hi) { // what hi = h2(a, b) leaves
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return h2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, __half2 b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), b);
+    return *reinterpret_cast<const uint32_t *>(&r);
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// HT: tiles of 8 rows (1 or 2); SPLIT: queries and probabilities in two f16 parts
+template <int HD, bool F8, int HT, bool SPLIT>
+__global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const __grid_constant__ KqAttnArgs a) {
+    constexpr int R = 8 * HT, ES = F8 ? 1 : 2, NG = F8 ? 2 : 1, KT = 16 * NG, U = NW * KT; // groups of 16 positions of a warp's step; positions of a unit
+    constexpr int KL = HD * ES / 64, VL = (HD * ES + 127) / 128;                           // 16-byte loads of a key and of a value
+    constexpr int KS = HD / 16, MT = HD / 16;                                              // steps of Q K^T, tiles of 16 dimensions of O^T
+    constexpr int QP = HD + 4;
+    __shared__ __align__(16) float q_s[R][QP];
+    __shared__ float c_s[R];
+    __shared__ __align__(16) float o_s[NW][R][HD];
+    __shared__ float m_s[NW][R], l_s[NW][R];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    KQ_PDL_ENTER();
+    KqRun run = kq_find_run<R, U, NT>(a);
+    int4 meta = make_int4(0, 0, 0, 0);
+    long long u = run.u0;
+    for (int s = run.s; u < run.u1 && s < a.b.n_seq; s++, run.off = 0) {
+        const KqSeq sq = kq_seq(a, s);
+        if (sq.t == 0) continue;
+        const int tiles = kq_tiles<R>(a, sq.t);
+        const long long per_head = kq_head_units<R, U>(a, sq);
+        int kh = (int)(run.off / per_head), tile = 0;
+        long long uo = run.off % per_head;
+        while (tile < tiles) { // the tile that the run begins in
+            const int n = kq_units<U>(kq_tile_keys<R>(a, sq, tile));
+            if (uo < n) break;
+            uo -= n;
+            tile++;
+        }
+        for (; kh < a.c.n_kv && u < run.u1; kh++, tile = 0)
+            for (; tile < tiles && u < run.u1; tile++, uo = 0) {
+                const int2 keys = kq_tile_keys<R>(a, sq, tile);
+                const int n_units = kq_units<U>(keys), take = (int)min((long long)n_units - uo, run.u1 - u), ub = (int)uo;
+                u += take;
+                // ---- the item's queries: rotated, normed, in shared memory
+                __syncthreads();
+                for (int r = warp; r < R; r += NW) {
+                    const int rr = tile * R + r, tok = rr / a.G, h = kh * a.G + rr % a.G;
+                    const bool ok = tok < sq.t;
+                    float amax = 0.f, x[HD / 32];
+#pragma unroll
+                    for (int i = 0; i < HD / 64; i++) {
+                        x[2 * i] = x[2 * i + 1] = 0.f;
+                        if (!ok) continue;
+                        const int pr = lane + 32 * i, d0 = a.turns.neox ? pr : 2 * pr, d1 = a.turns.neox ? pr + HD / 2 : 2 * pr + 1;
+                        const int64_t at = (int64_t)(sq.row0 + tok) * a.q_stride + (int64_t)h * HD;
+                        float v0, v1;
+                        if (a.type == B200_TYPE_F32) {
+                            v0 = ((const float *)a.q)[at + d0];
+                            v1 = ((const float *)a.q)[at + d1];
+                        } else if (a.type == B200_TYPE_F16) {
+                            v0 = __half2float(((const __half *)a.q)[at + d0]);
+                            v1 = __half2float(((const __half *)a.q)[at + d1]);
+                        } else {
+                            v0 = __bfloat162float(((const __nv_bfloat16 *)a.q)[at + d0]);
+                            v1 = __bfloat162float(((const __nv_bfloat16 *)a.q)[at + d1]);
+                        }
+                        if (a.turns.on) {
+                            const float2 cs = kq_turn(a.turns.f[pr], sq.pos(tok));
+                            const float w0 = v0 * cs.x - v1 * cs.y;
+                            v1 = v0 * cs.y + v1 * cs.x;
+                            v0 = w0;
+                        }
+                        x[2 * i] = v0;
+                        x[2 * i + 1] = v1;
+                        amax = fmaxf(amax, fmaxf(fabsf(v0), fabsf(v1)));
+                    }
+                    amax = kq_warp_max(amax);
+                    const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 252u);
+                    const float f = amax > 0.f ? __uint_as_float((254u - e) << 23) : 1.f;
+#pragma unroll
+                    for (int i = 0; i < HD / 64; i++) {
+                        const int pr = lane + 32 * i, d0 = a.turns.neox ? pr : 2 * pr, d1 = a.turns.neox ? pr + HD / 2 : 2 * pr + 1;
+                        q_s[r][d0] = x[2 * i] * f;
+                        q_s[r][d1] = x[2 * i + 1] * f;
+                    }
+                    if (lane == 0) c_s[r] = amax > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2;
+                }
+                __syncthreads();
+                uint32_t qh[KS][4], ql[SPLIT ? KS : 1][4];
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const int d = F8 ? 64 * (ks >> 2) + 16 * t4 + 4 * (ks & 3) : 32 * (ks >> 1) + 8 * t4 + 4 * (ks & 1);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (h >= HT) {
+                            qh[ks][h] = qh[ks][h + 2] = 0u;
+                            if (SPLIT) ql[ks][h] = ql[ks][h + 2] = 0u;
+                            continue;
+                        }
+                        const float4 v = *reinterpret_cast<const float4 *>(&q_s[g + 8 * h][d]);
+                        qh[ks][h] = h2(v.x, v.y);
+                        qh[ks][h + 2] = h2(v.z, v.w);
+                        if (SPLIT) {
+                            ql[ks][h] = h2_low(v.x, v.y, qh[ks][h]);
+                            ql[ks][h + 2] = h2_low(v.z, v.w, qh[ks][h + 2]);
+                        }
+                    }
+                }
+                float crow[HT], m[HT], l[HT], o[HT][MT][4];
+                int lim[HT]; // last position that row g (+ 8) sees
+#pragma unroll
+                for (int h = 0; h < HT; h++) {
+                    crow[h] = c_s[g + 8 * h];
+                    const int tok = min((tile * R + g + 8 * h) / a.G, sq.t - 1);
+                    lim[h] = sq.p0 < 0 ? -1 : sq.pos(tok);
+                    m[h] = -INFINITY;
+                    l[h] = 0.f;
+#pragma unroll
+                    for (int i = 0; i < MT; i++) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
+                }
+                const int see_all = sq.pos(tile * R / a.G);                                                                    // positions up to here every row sees ...
+                const int see_from = a.window > 0 ? sq.pos(min((tile * R + R - 1) / a.G, sq.t - 1)) - a.window + 1 : 0; // ... from here on
+                const int first_seen = a.window > 0 ? max(0, see_all - a.window + 1) : 0;                // before this one none does
+                const int bpp = a.c.page / KQ_PAGE_BLOCK;
+                const int64_t head_off = (int64_t)kh * a.c.page * HD * ES;
+                int pg[NG], inb[NG]; // page and block in it of this lane's step
+                for (int i = 0; i < take; i++) {
+                    if ((i & 31) == 0) { // a lane looks one of the next 32 steps up
+#pragma unroll
+                        for (int n = 0; n < NG; n++) {
+                            const int key = keys.x + (ub + i + lane) * U + warp * KT + 16 * n;
+                            pg[n] = -1;
+                            inb[n] = 0;
+                            if (i + lane < take && key < keys.y) {
+                                const int blk = key / KQ_PAGE_BLOCK, pi = blk / bpp;
+                                inb[n] = blk - pi * bpp;
+                                const int id = pi < a.c.table_len ? a.c.table[(int64_t)s * a.c.table_stride + pi] : -1;
+                                pg[n] = id >= 0 && id < a.c.n_pages ? id : -1;
+                            }
+                        }
+                    }
+                    const int key0 = keys.x + (ub + i) * U + warp * KT;
+                    if (key0 >= keys.y) continue; // warp-uniform
+                    uint4 kr[NG][2][KL], vr[NG][4][VL];
+                    float ksc[NG], vsc[NG];
+                    bool have[NG];
+#pragma unroll
+                    for (int n = 0; n < NG; n++) {
+                        const int p = __shfl_sync(0xffffffffu, pg[n], i & 31), ib = __shfl_sync(0xffffffffu, inb[n], i & 31);
+                        have[n] = p >= 0;
+                        ksc[n] = vsc[n] = 1.f;
+                        if (have[n]) {
+                            const int64_t off = (int64_t)p * a.c.page_bytes + head_off + (int64_t)ib * (KQ_PAGE_BLOCK * HD * ES);
+                            const uint8_t *kp = a.c.k + off, *vp = a.c.v + off;
+                            if (F8) {
+                                const int64_t at = ((int64_t)p * a.c.n_kv + kh) * bpp + ib;
+                                ksc[n] = a.c.ks[at];
+                                vsc[n] = a.c.vs[at];
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                                for (int j = 0; j < KL; j++) kr[n][nt][j] = ld16(kp + (8 * nt + g) * (HD * ES) + 64 * j + 16 * t4);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                const uint8_t *vrow = vp + (2 * t4 + (x & 1) + (x >> 1) * 8) * (HD * ES);
+                                if constexpr (HD * ES < 128) vr[n][x][0] = ld8(vrow + 8 * g);
+                                else {
+#pragma unroll
+                                    for (int j = 0; j < VL; j++) vr[n][x][j] = ld16(vrow + 128 * j + 16 * g);
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                                for (int j = 0; j < KL; j++) kr[n][nt][j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                            for (int x = 0; x < 4; x++)
+#pragma unroll
+                                for (int j = 0; j < VL; j++) vr[n][x][j] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    // ---- scores
+                    float sc[NG][2][4];
+#pragma unroll
+                    for (int n = 0; n < NG; n++)
+#pragma unroll
+                        for (int nt = 0; nt < 2; nt++) {
+                            float(&c)[4] = sc[n][nt];
+                            c[0] = c[1] = c[2] = c[3] = 0.f;
+#pragma unroll
+                            for (int ks = 0; ks < KS; ks++) {
+                                uint32_t b0, b1;
+                                if (F8) {
+                                    const uint32_t w = word(kr[n][nt][ks >> 2], ks & 3);
+                                    b0 = kq_e4m3x2_h2((uint16_t)w);
+                                    b1 = kq_e4m3x2_h2((uint16_t)(w >> 16));
+                                } else {
+                                    b0 = word(kr[n][nt][ks >> 1], 2 * (ks & 1));
+                                    b1 = word(kr[n][nt][ks >> 1], 2 * (ks & 1) + 1);
+                                }
+                                mma(c, qh[ks], b0, b1);
+                                if (SPLIT) mma(c, ql[SPLIT ? ks : 0], b0, b1);
+                            }
+                        }
+                    float mx[HT];
+#pragma unroll
+                    for (int h = 0; h < HT; h++) mx[h] = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < NG; n++) {
+                        const int kg = key0 + 16 * n;
+                        const bool all = have[n] && kg + 15 <= see_all && kg >= see_from;
+#pragma unroll
+                        for (int h = 0; h < HT; h++) {
+                            const float f = F8 ? crow[h] * ksc[n] : crow[h];
+#pragma unroll
+                            for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                                for (int j = 0; j < 2; j++) {
+                                    float &x = sc[n][nt][2 * h + j];
+                                    x *= f;
+                                    if (!all) {
+                                        const int key = kg + 8 * nt + 2 * t4 + j;
+                                        if (!have[n] || key > lim[h] || key >= keys.y || (a.window > 0 && key <= lim[h] - a.window)) x = -INFINITY;
+                                    }
+                                    mx[h] = fmaxf(mx[h], x);
+                                }
+                        }
+                        // a value that no row sees may hold anything: it must not meet a probability of 0
+                        if (have[n] && (kg + 16 > keys.y || kg < first_seen)) {
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                const int key = kg + 2 * t4 + (x & 1) + (x >> 1) * 8;
+                                if (key >= keys.y || key < first_seen) {
+#pragma unroll
+                                    for (int j = 0; j < VL; j++) vr[n][x][j] = make_uint4(0, 0, 0, 0);
+                                }
+                            }
+                        }
+                    }
+                    // ---- softmax
+                    float alpha[HT];
+                    bool same = true;
+                    uint32_t ph[NG][HT][2], pl[SPLIT ? NG : 1][HT][2];
+#pragma unroll
+                    for (int h = 0; h < HT; h++) {
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                        mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                        const float mn = fmaxf(m[h], mx[h]), sub = mn == -INFINITY ? 0.f : mn;
+                        alpha[h] = ex2(m[h] - sub); // nothing seen before: 2^-inf = 0
+                        same = same && m[h] == mn;
+                        m[h] = mn;
+                        float sum = 0.f;
+#pragma unroll
+                        for (int n = 0; n < NG; n++)
+#pragma unroll
+                            for (int nt = 0; nt < 2; nt++) {
+                                const float p0 = ex2(sc[n][nt][2 * h] - sub), p1 = ex2(sc[n][nt][2 * h + 1] - sub);
+                                sum += p0 + p1;
+                                ph[n][h][nt] = h2(p0, p1);
+                                if (SPLIT) pl[SPLIT ? n : 0][h][nt] = h2_low(p0, p1, ph[n][h][nt]);
+                            }
+                        l[h] = l[h] * alpha[h] + sum;
+                    }
+                    if (!__all_sync(0xffffffffu, same)) { // columns of O^T are rows 2 t4 and 2 t4 + 1: their factors sit in other lanes
+#pragma unroll
+                        for (int h = 0; h < HT; h++) {
+                            const float a0 = __shfl_sync(0xffffffffu, alpha[h], 8 * t4), a1 = __shfl_sync(0xffffffffu, alpha[h], 8 * t4 + 4);
+#pragma unroll
+                            for (int i = 0; i < MT; i++) {
+                                o[h][i][0] *= a0;
+                                o[h][i][1] *= a1;
+                                o[h][i][2] *= a0;
+                                o[h][i][3] *= a1;
+                            }
+                        }
+                    }
+                    // ---- values
+#pragma unroll
+                    for (int n = 0; n < NG; n++) {
+                        const __half2 vs2 = __float2half2_rn(vsc[n]);
+#pragma unroll
+                        for (int i = 0; i < MT; i++) {
+                            uint32_t va[4];
+                            if (F8) { // two tiles per word of four dimensions
+                                const uint32_t pick = i & 1 ? 0x7362u : 0x5140u;
+                                const uint32_t x = __byte_perm(word(vr[n][0][0], i >> 1), word(vr[n][1][0], i >> 1), pick);
+                                const uint32_t y = __byte_perm(word(vr[n][2][0], i >> 1), word(vr[n][3][0], i >> 1), pick);
+                                va[0] = mul_h2(kq_e4m3x2_h2((uint16_t)x), vs2);
+                                va[1] = mul_h2(kq_e4m3x2_h2((uint16_t)(x >> 16)), vs2);
+                                va[2] = mul_h2(kq_e4m3x2_h2((uint16_t)y), vs2);
+                                va[3] = mul_h2(kq_e4m3x2_h2((uint16_t)(y >> 16)), vs2);
+                            } else {
+                                const uint32_t w0 = word(vr[n][0][i >> 2], i & 3), w1 = word(vr[n][1][i >> 2], i & 3);
+                                const uint32_t w2 = word(vr[n][2][i >> 2], i & 3), w3 = word(vr[n][3][i >> 2], i & 3);
+                                va[0] = __byte_perm(w0, w1, 0x5410u);
+                                va[1] = __byte_perm(w0, w1, 0x7632u);
+                                va[2] = __byte_perm(w2, w3, 0x5410u);
+                                va[3] = __byte_perm(w2, w3, 0x7632u);
+                            }
+#pragma unroll
+                            for (int h = 0; h < HT; h++) {
+                                mma(o[h][i], va, ph[n][h][0], ph[n][h][1]);
+                                if (SPLIT) mma(o[h][i], va, pl[SPLIT ? n : 0][h][0], pl[SPLIT ? n : 0][h][1]);
+                            }
+                        }
+                    }
+                }
+                // ---- the four warps' rows, joined in warp order
+#pragma unroll
+                for (int h = 0; h < HT; h++) {
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                    if (t4 == 0) {
+                        m_s[warp][g + 8 * h] = m[h];
+                        l_s[warp][g + 8 * h] = l[h];
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        const int d = F8 ? (HD / 8) * g + 2 * i : 64 * (i >> 2) + 8 * g + 2 * (i & 3);
+                        *reinterpret_cast<float2 *>(&o_s[warp][8 * h + 2 * t4][d]) = make_float2(o[h][i][0], o[h][i][2]);
+                        *reinterpret_cast<float2 *>(&o_s[warp][8 * h + 2 * t4 + 1][d]) = make_float2(o[h][i][1], o[h][i][3]);
+                    }
+                }
+                __syncthreads();
+                const bool whole = ub == 0 && take == n_units;
+                const int slot = 2 * blockIdx.x + (ub == 0 ? 1 : 0);
+                float *po = a.part + (int64_t)slot * R * (HD + 2), *pml = po + R * HD;
+                if (ub == 0 && !whole) {
+                    const int per = (int)min((long long)0x7fffffff, run.u1 - run.u0); // a CTA whose item goes on has a full run
+                    meta = make_int4(1 + (int)(((long long)n_units - take + per - 1) / per), s, kh, tile);
+                }
+                for (int i = tid; i < R * (HD / 2); i += NT) {
+                    const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
+                    const int rr = tile * R + r, tok = rr / a.G;
+                    if (tok >= sq.t) continue;
+                    float mm = m_s[0][r];
+#pragma unroll
+                    for (int w = 1; w < NW; w++) mm = fmaxf(mm, m_s[w][r]);
+                    const float sub = mm == -INFINITY ? 0.f : mm;
+                    float x = 0.f, y = 0.f, ll = 0.f;
+#pragma unroll
+                    for (int w = 0; w < NW; w++) {
+                        const float f = ex2(m_s[w][r] - sub);
+                        const float2 v = *reinterpret_cast<const float2 *>(&o_s[w][r][d]);
+                        x += f * v.x;
+                        y += f * v.y;
+                        ll += f * l_s[w][r];
+                    }
+                    if (whole) {
+                        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+                        kq_st2_type(a.type, a.out, (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(kh * a.G + rr % a.G) * HD + d, x * inv, y * inv);
+                    } else {
+                        *reinterpret_cast<float2 *>(po + r * HD + d) = make_float2(x, y);
+                        if (d == 0) *reinterpret_cast<float2 *>(pml + 2 * r) = make_float2(mm, ll);
+                    }
+                }
+            }
+    }
+    if (tid == 0) a.meta[blockIdx.x] = meta;
+}
+
+// CTA (b, row): one row of the item that begins in CTA b of the attention kernel and goes on in the next pieces - 1 of them.
+// 512 threads: groups of HD threads take every group-th piece.
+template <int HD> __global__ void __launch_bounds__(512) pages_combine_kernel(const __grid_constant__ KqAttnArgs a, int R) {
+    constexpr int NGRP = 512 / HD;
+    __shared__ float x_s[NGRP][HD], l_s[NGRP], m_s[16];
+    KQ_PDL_ENTER();
+    const int4 meta = a.meta[blockIdx.x];
+    if (meta.x == 0) return;
+    const KqSeq sq = kq_seq(a, meta.y);
+    const int r = blockIdx.y, rr = meta.w * R + r, tok = rr / a.G;
+    if (tok >= sq.t) return;
+    const int tid = threadIdx.x, d = tid % HD, grp = tid / HD;
+    const int64_t slot_floats = (int64_t)R * (HD + 2);
+    // piece 0 is slot 2 b + 1, piece i slot 2 (b + i)
+    auto piece = [&](int i) { return a.part + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * slot_floats; };
+    float mm = -INFINITY;
+    for (int i = tid; i < meta.x; i += 512) mm = fmaxf(mm, piece(i)[R * HD + 2 * r]);
+    mm = kq_warp_max(mm);
+    if ((tid & 31) == 0) m_s[tid >> 5] = mm;
+    __syncthreads();
+    mm = m_s[0];
+#pragma unroll
+    for (int w = 1; w < 16; w++) mm = fmaxf(mm, m_s[w]);
+    const float sub = mm == -INFINITY ? 0.f : mm;
+    float x = 0.f, l = 0.f;
+    for (int i0 = grp; i0 < meta.x; i0 += 8 * NGRP) {
+        float v[8];
+        float2 ml[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int i = i0 + j * NGRP;
+            v[j] = 0.f;
+            ml[j] = make_float2(-INFINITY, 0.f);
+            if (i < meta.x) {
+                const float *p = piece(i);
+                v[j] = p[r * HD + d];
+                ml[j] = *reinterpret_cast<const float2 *>(p + R * HD + 2 * r);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float f = ex2(ml[j].x - sub);
+            x += f * v[j];
+            l += f * ml[j].y;
+        }
+    }
+    x_s[grp][d] = x;
+    if (d == 0) l_s[grp] = l;
+    __syncthreads();
+    if (tid >= HD / 2) return;
+    float2 y = make_float2(0.f, 0.f);
+    float ll = 0.f;
+#pragma unroll
+    for (int i = 0; i < NGRP; i++) {
+        y.x += x_s[i][2 * tid];
+        y.y += x_s[i][2 * tid + 1];
+        ll += l_s[i];
+    }
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    kq_st2_type(a.type, a.out, (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(meta.z * a.G + rr % a.G) * HD + 2 * tid, y.x * inv, y.y * inv);
+}
+
+template <int HD, bool F8, int HT, bool SPLIT> b200_status launch(const KqAttnArgs &a, int ctas, cudaStream_t st) {
+    kq_launch(pages_decode_kernel<HD, F8, HT, SPLIT>, ctas, NT, 0, st, a);
+    KQ_COUNT_LAUNCH();
+    KQ_LAUNCH_CHECK();
+    return B200_OK;
+}
+template <int HD, bool F8> b200_status launch(const KqAttnArgs &a, int ht, bool split, int ctas, cudaStream_t st) {
+    if (ht == 1) return split ? launch<HD, F8, 1, true>(a, ctas, st) : launch<HD, F8, 1, false>(a, ctas, st);
+    return split ? launch<HD, F8, 2, true>(a, ctas, st) : launch<HD, F8, 2, false>(a, ctas, st);
+}
+
+constexpr size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+} // namespace
+
+b200_status kq_pages_combine(const KqAttnArgs &a, int hd, int R, int ctas, cudaStream_t st) {
+    const dim3 grid((unsigned)ctas, (unsigned)R);
+    kq_launch(hd == 128 ? pages_combine_kernel<128> : pages_combine_kernel<64>, grid, 512, 0, st, a, R);
+    KQ_COUNT_LAUNCH();
+    KQ_LAUNCH_CHECK();
+    return B200_OK;
+}
+
+size_t kq_pages_decode_scratch(int hd) {
+    const size_t ctas = (size_t)kq_sm_count() * MAX_CTAS_PER_SM;
+    return up256(ctas * sizeof(int4)) + ctas * 2 * 16 * (hd + 2) * sizeof(float);
+}
+
+b200_status kq_pages_decode(KqAttnArgs a, bool f8, int hd, int64_t most, uint8_t *scratch, cudaStream_t st) {
+    const bool split = a.type == B200_TYPE_F32;
+    const int ht = most <= 8 ? 1 : 2, ctas = kq_sm_count() * (ht == 1 ? 3 : 2);
+    a.meta = (int4 *)scratch;
+    a.part = (float *)(scratch + up256((size_t)kq_sm_count() * MAX_CTAS_PER_SM * sizeof(int4)));
+    if (hd == 128) KQ_TRY(f8 ? (launch<128, true>(a, ht, split, ctas, st)) : (launch<128, false>(a, ht, split, ctas, st)));
+    else KQ_TRY(f8 ? (launch<64, true>(a, ht, split, ctas, st)) : (launch<64, false>(a, ht, split, ctas, st)));
+    return kq_pages_combine(a, hd, 8 * ht, ctas, st);
+}
+
+extern "C" {
+
+size_t b200_attention_pages_scratch_bytes(const b200_kv_pages *cache, int32_t n_head, int32_t max_rows) {
+    (void)n_head, (void)max_rows;
+    if (!cache || (cache->head_dim != 64 && cache->head_dim != 128)) return 0;
+    return kq_pages_decode_scratch(cache->head_dim);
+}
+
+b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type, const void *q, int64_t q_stride, int32_t n_head,
+                                 int32_t max_rows, float theta, int32_t neox, int32_t window, float scale, void *out, int64_t out_stride, void *scratch,
+                                 size_t scratch_bytes, void *stream) {
+    KqAttnArgs a = {};
+    KQ_TRY(kq_pages_check("attention_pages", cache, batch, &a.c, &a.b));
+    KQ_REQUIRE(n_head >= 1 && n_head <= 4096 && n_head % cache->n_kv == 0, "attention_pages: %d query heads on %d KV heads", n_head, cache->n_kv);
+    KQ_REQUIRE(theta >= 0.f && isfinite(theta), "attention_pages: rotation base %g", theta);
+    KQ_REQUIRE(scale >= 0.f && isfinite(scale), "attention_pages: scale %g", scale);
+    KQ_REQUIRE(a.b.rows * (int64_t)n_head <= 0x3fffffff, "attention_pages: %d rows of %d heads", a.b.rows, n_head);
+    KQ_REQUIRE(window >= 0 && max_rows >= 0, "attention_pages: window %d, rows %d", window, max_rows);
+    if (a.b.rows == 0 || a.b.n_seq == 0) return B200_OK;
+    const int hd = cache->head_dim;
+    KQ_TRY(kq_rows_check("attention_pages", "queries", q, type, q_stride, (int64_t)n_head * hd));
+    KQ_TRY(kq_rows_check("attention_pages", "results", out, type, out_stride, (int64_t)n_head * hd));
+    KQ_REQUIRE(scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= b200_attention_pages_scratch_bytes(cache, n_head, max_rows),
+               "attention_pages: scratch of %zu bytes, 16-byte aligned, required", b200_attention_pages_scratch_bytes(cache, n_head, max_rows));
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.type = type;
+    a.n_head = n_head;
+    a.G = n_head / cache->n_kv;
+    a.window = window;
+    a.t_lo = 1;
+    a.t_hi = INT64_MAX;
+    a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)hd)) * 1.4426950408889634f;
+    a.turns = kq_turns(theta, neox, hd);
+    return kq_pages_decode(a, cache->type == B200_TYPE_F8_E4M3, hd, (int64_t)(max_rows > 0 ? max_rows : 1) * a.G, (uint8_t *)scratch, (cudaStream_t)stream);
+}
+
+} // extern "C"

@@ -1,0 +1,105 @@
+// How the kernels of b200_attention_pages share a ragged batch: the lengths are on the device, so every CTA works its part out itself.
+//
+// An item is one tile of R rows (row i of a sequence and KV head: new token i / G, query head i % G) of one sequence and KV head; its keys
+// are cut into units of U positions.  All units of all items in order (sequence, head, tile, key) are cut into equal runs, one per CTA, so that
+// the longest sequence does not decide how long the launch takes.  A CTA's run is at most the end of one item (its partial result goes into slot
+// 2 cta), whole items (results go out), and the beginning of another (slot 2 cta + 1); meta[cta] describes the item that begins there and
+// goes on in other CTAs, and the combining kernel joins its slots in order.  Nothing depends on timing.
+#pragma once
+#include "kq_pages.cuh"
+
+struct KqAttnArgs {
+    KqPages c;
+    KqBatch b;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    uint32_t type;
+    int32_t n_head, G, window;
+    int64_t t_lo, t_hi; // sequences with t_lo <= rows x G <= t_hi are this kernel's
+    float scale_log2;
+    KqTurns turns;
+    float *part; // [2 CTAs][R][HD + 2]: unnormalised rows, then (maximum, sum) of each
+    int4 *meta;  // [CTAs]: pieces (0: none), sequence, KV head, tile
+};
+
+#ifdef __CUDACC__
+struct KqSeq {
+    int t, p0, row0;
+    __device__ __forceinline__ int pos(int tok) const { return (int)min((int64_t)p0 + tok, (int64_t)0x7fffffff); }
+};
+__device__ __forceinline__ KqSeq kq_seq(const KqAttnArgs &a, int s) {
+    const int2 r = kq_seq_rows(a.b, s);
+    const int64_t n = (int64_t)(r.y - r.x) * a.G;
+    return KqSeq{n >= a.t_lo && n <= a.t_hi ? r.y - r.x : 0, a.b.pos0[s], r.x};
+}
+template <int R> __device__ __forceinline__ int kq_tiles(const KqAttnArgs &a, int t) { return (int)(((int64_t)t * a.G + R - 1) / R); }
+// positions [x, y) that some row of the tile sees; x is a multiple of 16
+template <int R> __device__ __forceinline__ int2 kq_tile_keys(const KqAttnArgs &a, const KqSeq &q, int tile) {
+    const int first = (int)((int64_t)tile * R / a.G), last = (int)min((int64_t)q.t - 1, ((int64_t)tile * R + R - 1) / a.G);
+    const int64_t cap = (int64_t)a.c.table_len * a.c.page;
+    const int hi = q.p0 < 0 ? 0 : (int)min((int64_t)q.p0 + last + 1, cap);
+    const int lo = a.window > 0 ? (int)max((int64_t)0, (int64_t)q.p0 + first - a.window + 1) & ~(KQ_PAGE_BLOCK - 1) : 0;
+    return make_int2(min(lo, hi & ~(KQ_PAGE_BLOCK - 1)), hi);
+}
+template <int U> __device__ __forceinline__ int kq_units(int2 keys) { return max(1, (keys.y - keys.x + U - 1) / U); }
+template <int R, int U> __device__ __forceinline__ long long kq_head_units(const KqAttnArgs &a, const KqSeq &q) {
+    long long n = 0;
+    const int tiles = kq_tiles<R>(a, q.t);
+    for (int i = 0; i < tiles; i++) n += kq_units<U>(kq_tile_keys<R>(a, q, i));
+    return n;
+}
+
+// this CTA's run of units: [u0, u1), beginning `off` units into sequence s
+struct KqRun {
+    long long u0, u1, off;
+    int s;
+};
+template <int R, int U, int NT> __device__ KqRun kq_find_run(const KqAttnArgs &a) {
+    __shared__ long long warp_sum[NT / 32], s_off;
+    __shared__ int s_seq;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int each = (a.b.n_seq + NT - 1) / NT, i0 = min(a.b.n_seq, tid * each), i1 = min(a.b.n_seq, i0 + each);
+    long long sum = 0;
+    for (int i = i0; i < i1; i++) sum += kq_head_units<R, U>(a, kq_seq(a, i)) * a.c.n_kv;
+    long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) warp_sum[warp] = inc;
+    if (tid == 0) s_seq = a.b.n_seq;
+    __syncthreads();
+    long long before = inc - sum, total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; w++) {
+        if (w < warp) before += warp_sum[w];
+        total += warp_sum[w];
+    }
+    const long long per = max(1ll, (total + gridDim.x - 1) / (long long)gridDim.x), u0 = per * blockIdx.x;
+    if (u0 >= before && u0 < before + sum) {
+        long long off = u0 - before;
+        for (int i = i0; i < i1; i++) {
+            const long long n = kq_head_units<R, U>(a, kq_seq(a, i)) * a.c.n_kv;
+            if (off < n) {
+                s_seq = i;
+                s_off = off;
+                break;
+            }
+            off -= n;
+        }
+    }
+    __syncthreads();
+    KqRun r{u0, min(total, u0 + per), 0, s_seq};
+    if (r.s < a.b.n_seq) r.off = s_off;
+    else r.u1 = r.u0;
+    return r;
+}
+#endif
+
+// joins the pieces of split items; grid (CTAs of the attention kernel, rows of a tile)
+b200_status kq_pages_combine(const KqAttnArgs &a, int hd, int R, int ctas, cudaStream_t st);
+// sequences of few rows (any number is right), and its workspace
+size_t kq_pages_decode_scratch(int hd);
+b200_status kq_pages_decode(KqAttnArgs a, bool f8, int hd, int64_t most, uint8_t *scratch, cudaStream_t st);
