@@ -376,6 +376,7 @@ int kq_gemm_error_fetch();
 int kq_attn_tc_error_fetch();
 int kq_gemm_bf16_error_fetch();
 int kq_prompt_attn_error_fetch();
+int kq_pages_error_fetch();
 int kq_state_error_fetch();
 int kq_state_chunk_error_fetch();
 int kq_device_wait_errors(); // all of the above in one code

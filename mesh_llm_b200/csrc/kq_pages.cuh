@@ -79,6 +79,9 @@ template <> __device__ __forceinline__ float2 kq_ld2<__nv_bfloat16>(const __nv_b
 __device__ __forceinline__ float2 kq_ld2_type(uint32_t type, const void *p, int64_t at) {
     return type == B200_TYPE_F32 ? kq_ld2((const float *)p + at) : type == B200_TYPE_F16 ? kq_ld2((const __half *)p + at) : kq_ld2((const __nv_bfloat16 *)p + at);
 }
+__device__ __forceinline__ float kq_ld1_type(uint32_t type, const void *p, int64_t at) {
+    return type == B200_TYPE_F32 ? ((const float *)p)[at] : type == B200_TYPE_F16 ? __half2float(((const __half *)p)[at]) : __bfloat162float(((const __nv_bfloat16 *)p)[at]);
+}
 __device__ __forceinline__ void kq_st2_type(uint32_t type, void *p, int64_t at, float a, float b) {
     if (type == B200_TYPE_F32) *reinterpret_cast<float2 *>((float *)p + at) = make_float2(a, b);
     else if (type == B200_TYPE_F16) *reinterpret_cast<__half2 *>((__half *)p + at) = __floats2half2_rn(a, b);

@@ -51,9 +51,6 @@ template <int HD, bool F8, int N, bool SPLIT> struct Block {
         if (!split) return 2 * P * lane + e;
         return HD == 128 ? (e >> 1) * 64 + 2 * lane + (e & 1) : e * 32 + lane;
     }
-    __device__ static float scalar(uint32_t type, const void *p, int64_t at) {
-        return type == B200_TYPE_F32 ? ((const float *)p)[at] : type == B200_TYPE_F16 ? __half2float(((const __half *)p)[at]) : __bfloat162float(((const __nv_bfloat16 *)p)[at]);
-    }
     __device__ static void load(float (&x)[N][2 * P], const Rows &r, const void *p, int64_t at, int64_t stride, int cnt, int lane) {
 #pragma unroll
         for (int j = 0; j < N; j++) {
@@ -64,8 +61,8 @@ template <int HD, bool F8, int N, bool SPLIT> struct Block {
             }
             const int64_t o = at + j * stride;
             if (HD == 64 && split) {
-                x[j][0] = scalar(r.type, p, o + lane);
-                x[j][1] = scalar(r.type, p, o + 32 + lane);
+                x[j][0] = kq_ld1_type(r.type, p, o + lane);
+                x[j][1] = kq_ld1_type(r.type, p, o + 32 + lane);
                 continue;
             }
 #pragma unroll
@@ -224,7 +221,9 @@ KqTurns kq_turns(float theta, int neox, int hd) {
     KqTurns t;
     t.on = theta > 0.f;
     t.neox = neox != 0;
-    for (int i = 0; i < 64; i++) t.f[i] = t.on && i < hd / 2 ? pow((double)theta, -2.0 * i / hd) / 6.283185307179586476925 : 0.0;
+    const double ratio = t.on ? pow((double)theta, -2.0 / hd) : 0.0; // one power: 63 products are off by 10^-14
+    double f = t.on ? 1.0 / 6.283185307179586476925 : 0.0;
+    for (int i = 0; i < 64; i++, f *= ratio) t.f[i] = i < hd / 2 ? f : 0.0;
     return t;
 }
 

@@ -15,6 +15,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace {
 
 constexpr int NT = 128, NW = NT / 32;
@@ -100,17 +102,7 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                         if (!ok) continue;
                         const int pr = lane + 32 * i, d0 = a.turns.neox ? pr : 2 * pr, d1 = a.turns.neox ? pr + HD / 2 : 2 * pr + 1;
                         const int64_t at = (int64_t)(sq.row0 + tok) * a.q_stride + (int64_t)h * HD;
-                        float v0, v1;
-                        if (a.type == B200_TYPE_F32) {
-                            v0 = ((const float *)a.q)[at + d0];
-                            v1 = ((const float *)a.q)[at + d1];
-                        } else if (a.type == B200_TYPE_F16) {
-                            v0 = __half2float(((const __half *)a.q)[at + d0]);
-                            v1 = __half2float(((const __half *)a.q)[at + d1]);
-                        } else {
-                            v0 = __bfloat162float(((const __nv_bfloat16 *)a.q)[at + d0]);
-                            v1 = __bfloat162float(((const __nv_bfloat16 *)a.q)[at + d1]);
-                        }
+                        float v0 = kq_ld1_type(a.type, a.q, at + d0), v1 = kq_ld1_type(a.type, a.q, at + d1);
                         if (a.turns.on) {
                             const float2 cs = kq_turn(a.turns.f[pr], sq.pos(tok));
                             const float w0 = v0 * cs.x - v1 * cs.y;
@@ -481,6 +473,10 @@ template <int HD, bool F8> b200_status launch(const KqAttnArgs &a, int ht, bool 
     return split ? launch<HD, F8, 2, true>(a, ctas, st) : launch<HD, F8, 2, false>(a, ctas, st);
 }
 
+// Sequences of up to FEW rows of a KV head go to the kernel above, longer ones to the one for prompts, where the caller says there are any
+constexpr int64_t FEW = 64;
+bool prompts(int64_t G, int64_t max_rows) { return G * max_rows > FEW; }
+
 constexpr size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 } // namespace
@@ -511,9 +507,10 @@ b200_status kq_pages_decode(KqAttnArgs a, bool f8, int hd, int64_t most, uint8_t
 extern "C" {
 
 size_t b200_attention_pages_scratch_bytes(const b200_kv_pages *cache, int32_t n_head, int32_t max_rows) {
-    (void)n_head, (void)max_rows;
-    if (!cache || (cache->head_dim != 64 && cache->head_dim != 128)) return 0;
-    return kq_pages_decode_scratch(cache->head_dim);
+    if (!cache || (cache->head_dim != 64 && cache->head_dim != 128) || cache->n_kv < 1 || n_head < 1) return 0;
+    const size_t few = kq_pages_decode_scratch(cache->head_dim);
+    // the two kernels run one after the other: they share the room
+    return prompts(n_head / cache->n_kv, max_rows) ? std::max(few, kq_pages_prompt_scratch(cache->head_dim)) : few;
 }
 
 b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type, const void *q, int64_t q_stride, int32_t n_head,
@@ -544,7 +541,13 @@ b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_bat
     a.t_hi = INT64_MAX;
     a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)hd)) * 1.4426950408889634f;
     a.turns = kq_turns(theta, neox, hd);
-    return kq_pages_decode(a, cache->type == B200_TYPE_F8_E4M3, hd, (int64_t)(max_rows > 0 ? max_rows : 1) * a.G, (uint8_t *)scratch, (cudaStream_t)stream);
+    const bool f8 = cache->type == B200_TYPE_F8_E4M3, many = prompts(a.G, max_rows);
+    if (many) a.t_hi = FEW;
+    if (!many || a.b.n_seq > 1) KQ_TRY(kq_pages_decode(a, f8, hd, std::min<int64_t>(FEW, (int64_t)std::max(max_rows, 1) * a.G), (uint8_t *)scratch, (cudaStream_t)stream));
+    if (!many) return B200_OK;
+    a.t_lo = a.b.n_seq > 1 ? FEW + 1 : 1;
+    a.t_hi = INT64_MAX;
+    return kq_pages_prompt(a, f8, hd, (uint8_t *)scratch, (cudaStream_t)stream);
 }
 
 } // extern "C"

@@ -1,0 +1,722 @@
+// Attention of many new rows per sequence over paged keys and values (b200_attention_pages): prompts, on the 5th-generation tensor cores.
+//
+// A CTA works on two tiles of 128 rows (row i of a sequence and KV head: token i / G, head i % G) that share every tile of 128 keys: while
+// the tensor cores multiply for one, the softmax warps of the other work.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with S (columns
+// 0 and 128) and O (256 and 384) in TMEM; a softmax thread owns a row: it writes its probabilities over scores that it has read, as f16, which
+// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 8 in base 2 (a
+// probability then is at most 2^8, far from f16's end).  f32 queries go in as two f16 parts, and so do their probabilities; f16 queries, which the rotation makes longer than f16, go in as two.  As in the kernel for few rows a query row is
+// divided by the power of two of its largest element.
+//
+// K and V tiles go through a ring in the order K0 V0 K1 V1 ...; f16 pages arrive by tiled TMA, 64 dimensions x 16 .. 128 positions of a page
+// to a box, with the 128-byte swizzle that both products read (V as an MN-major operand), pages that are not there as the zeros of an
+// out-of-range coordinate; e4m3 pages arrive as raw rows by bulk copies and four warps turn them into the f16 tile of what they stand for.
+//
+// Bound by the tensor pipe (4 x 512 clocks for 256 rows x 128 keys at head_dim 128) and as much by the exponentials (16 a clock: 2 x 1024).  Units are
+// shared out evenly over one CTA per SM (kq_pages_sched.cuh).  Every wait is bounded: on a time-out the kernel records
+// an error, lets its copies land, frees its TMEM and returns.
+#include "kq_pages_sched.cuh"
+
+#include <cuda.h>
+#include <math.h>
+#include <string.h>
+
+b200_status kq_tmap_encode(void *map128, int elem_bytes, int rank, const void *base, const uint64_t *dims, const uint64_t *strides_bytes, const uint32_t *box, int swizzle128);
+
+namespace {
+
+constexpr int R = 256, BK = 128, NSOFT = 256;
+constexpr uint64_t LIMIT = 5 * KQ_WAIT_LIMIT_NS;
+constexpr uint32_t COL_S = 0, COL_O = 256;
+
+__device__ int g_pages_error;
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// shared-memory matrix descriptor, 128-byte swizzle
+__device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+constexpr int HALF = BK * 128; // 128 rows of 64 dimensions
+// K-major operand (Q, K^T): rows of 128 bytes, groups of 8 rows 1024 bytes apart; step s of 16 dimensions
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int s) { return make_desc(tile + (s >> 2) * HALF + (s & 3) * 32, 16, 1024); }
+// MN-major operand (V): atoms of 64 dimensions HALF apart, groups of 8 positions 1024 bytes apart; step s of 16 positions
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int s) { return make_desc(tile + s * 2048, HALF, 1024); }
+__device__ __forceinline__ constexpr uint32_t idesc(bool b_mn, int n) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+                 "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+                 "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t h2_low(float a, float b, uint32_t hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return h2(a - f.x, b - f.y);
+}
+
+template <int HD, bool F8, int QS> struct Layout {
+    static constexpr int TILE = BK * HD * 2, RAW = BK * HD;                     // an f16 tile of the ring, a raw e4m3 tile
+    static constexpr int Q = 2 * QS * TILE;                                     // [part][tile of rows]
+    static constexpr int NR = F8 ? (HD == 128 && QS == 2 ? 2 : 4) : 0;          // raw tiles
+    static constexpr int FREE = 224 * 1024 - Q - NR * RAW, NS0 = FREE / TILE, NS = NS0 > 6 ? 6 : NS0; // ring slots
+    static constexpr int RING = Q, RAWS = Q + NS * TILE, TOTAL = RAWS + NR * RAW + 1024;
+    static_assert(NS >= 2, "the ring holds a tile of keys and one of values");
+};
+constexpr int MAX_SLOTS = 6;
+
+struct Shared {
+    uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_done, q_ready;
+    float crow[R];
+    uint32_t tmem;
+    int abort;
+};
+
+// one CTA's pieces in order; every role walks them by itself
+struct Walk {
+    KqSeq sq;
+    int s, kh, tile, tiles, ub, take, n_units;
+    int2 keys;
+    long long u, u1, uo;
+    __device__ void start(const KqAttnArgs &a, const KqRun &run) {
+        u = run.u0;
+        u1 = run.u1;
+        s = run.s;
+        if (u >= u1) return;
+        sq = kq_seq(a, s);
+        const long long per_head = kq_head_units<R, BK>(a, sq);
+        kh = (int)(run.off / per_head);
+        uo = run.off % per_head;
+        tiles = kq_tiles<R>(a, sq.t);
+        for (tile = 0;; tile++) {
+            n_units = kq_units<BK>(kq_tile_keys<R>(a, sq, tile));
+            if (uo < n_units || tile + 1 >= tiles) break;
+            uo -= n_units;
+        }
+    }
+    // the next piece; false: no more
+    __device__ bool next(const KqAttnArgs &a) {
+        if (u >= u1) return false;
+        while (tile >= tiles) {
+            tile = 0;
+            if (++kh >= a.c.n_kv) {
+                kh = 0;
+                do {
+                    if (++s >= a.b.n_seq) return false;
+                    sq = kq_seq(a, s);
+                } while (sq.t == 0);
+                tiles = kq_tiles<R>(a, sq.t);
+            }
+        }
+        keys = kq_tile_keys<R>(a, sq, tile);
+        n_units = kq_units<BK>(keys);
+        take = (int)min((long long)n_units - uo, u1 - u);
+        ub = (int)uo;
+        u += take;
+        return true;
+    }
+    __device__ void done() {
+        tile++;
+        uo = 0;
+    }
+};
+
+// codes of 8 dimensions as f16 numbers times the block's scale
+__device__ __forceinline__ uint4 decode8(uint32_t lo, uint32_t hi, __half2 s) {
+    auto two = [&](uint32_t v) {
+        const uint32_t h = kq_e4m3x2_h2((uint16_t)v);
+        const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&h), s);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    };
+    return make_uint4(two(lo), two(lo >> 16), two(hi), two(hi >> 16));
+}
+
+template <int HD, bool F8, int QS, int PS>
+__global__ void __launch_bounds__(F8 ? 512 : 384, 1)
+    pages_prompt_kernel(const __grid_constant__ KqAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box_rows) {
+    using L = Layout<HD, F8, QS>;
+    constexpr int NS = L::NS, NR = L::NR > 0 ? L::NR : 1, NT = F8 ? 512 : 384;
+    extern __shared__ __align__(1024) uint8_t sm_raw[];
+    uint8_t *sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
+    __shared__ Shared sh;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        auto init = [](uint64_t &b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&b)), "r"(n)); };
+        for (int i = 0; i < MAX_SLOTS; i++) {
+            init(sh.full[i], F8 ? 128 : 1);
+            init(sh.empty[i], 1);
+        }
+        for (int i = 0; i < 4; i++) {
+            init(sh.raw_full[i], 1);
+            init(sh.raw_empty[i], 128);
+        }
+        for (int i = 0; i < 2; i++) {
+            init(sh.s_ready[i], 1);
+            init(sh.p_ready[i], 128);
+        }
+        init(sh.o_done, 1);
+        init(sh.q_ready, NSOFT);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        sh.abort = 0;
+    }
+    before_sync();
+    __syncthreads();
+    after_sync();
+    const uint32_t tmem = sh.tmem;
+    volatile int *abort = &sh.abort;
+    auto wait = [&](uint64_t &bar, uint32_t parity, int code) {
+        if (!*abort && !kq_mbar_wait(smem_u32(&bar), parity, LIMIT)) {
+            *abort = 1;
+            atomicExch(&g_pages_error, code);
+        }
+    };
+    KQ_PDL_ENTER();
+    const KqRun run = kq_find_run<R, BK, NT>(a);
+    Walk w;
+    w.start(a, run);
+    const int bpp = a.c.page / KQ_PAGE_BLOCK;
+    int4 meta = make_int4(0, 0, 0, 0);
+
+    if (warp == 8) {
+        // ---------------------------------------------------------------- products
+        if (lane == 0) {
+            uint32_t tile_n = 0, pieces = 0, units = 0; // ring tiles, pieces and units so far
+            while (w.next(a)) {
+                wait(sh.q_ready, pieces & 1, 1);
+                after_sync();
+                const uint32_t ring = smem_u32(sm + L::RING), q0 = smem_u32(sm);
+                auto slot = [&](uint32_t t) { return ring + (t % NS) * L::TILE; };
+                auto scores = [&](int half, uint32_t t) {
+                    if (*abort) return;
+#pragma unroll
+                    for (int p = 0; p < QS; p++)
+#pragma unroll
+                        for (int s = 0; s < HD / 16; s++)
+                            mma_ss(tmem + COL_S + 128 * half, desc_k(q0 + (2 * p + half) * L::TILE, s), desc_k(slot(t), s), idesc(false, BK), p + s > 0);
+                };
+                auto values = [&](int half, uint32_t t, bool first) {
+                    if (*abort) return;
+#pragma unroll
+                    for (int p = 0; p < PS; p++)
+#pragma unroll
+                        for (int s = 0; s < BK / 16; s++)
+                            mma_ts(tmem + COL_O + 128 * half, tmem + COL_S + 128 * half + 64 * (s >> 2) + 32 * p + 8 * (s & 3), desc_mn(slot(t), s), idesc(true, HD), !(first && p + s == 0));
+                };
+                wait(sh.full[tile_n % NS], (tile_n / NS) & 1, 2);
+                after_sync();
+                scores(0, tile_n);
+                commit(smem_u32(&sh.s_ready[0]));
+                scores(1, tile_n);
+                commit(smem_u32(&sh.s_ready[1]));
+                commit(smem_u32(&sh.empty[tile_n % NS]));
+                for (int i = 0; i < w.take; i++) {
+                    const uint32_t v = tile_n + 1, k = tile_n + 2;
+                    const bool more = i + 1 < w.take;
+                    wait(sh.p_ready[0], units & 1, 3);
+                    wait(sh.full[v % NS], (v / NS) & 1, 4);
+                    after_sync();
+                    values(0, v, i == 0);
+                    if (more) {
+                        wait(sh.full[k % NS], (k / NS) & 1, 5);
+                        after_sync();
+                        scores(0, k);
+                        commit(smem_u32(&sh.s_ready[0]));
+                    }
+                    wait(sh.p_ready[1], units & 1, 6);
+                    after_sync();
+                    values(1, v, i == 0);
+                    commit(smem_u32(&sh.empty[v % NS]));
+                    if (more) {
+                        scores(1, k);
+                        commit(smem_u32(&sh.s_ready[1]));
+                        commit(smem_u32(&sh.empty[k % NS]));
+                    }
+                    tile_n += 2;
+                    units++;
+                }
+                commit(smem_u32(&sh.o_done));
+                pieces++;
+                w.done();
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---------------------------------------------------------------- copies: a lane per box
+        const int boxes = BK / box_rows, halves = F8 ? 1 : HD / 64, box = lane / halves, half = lane % halves;
+        uint32_t tile_n = 0;
+        while (w.next(a)) {
+            const int seen = a.window > 0 ? max(0, w.sq.pos(w.tile * R / a.G) - a.window + 1) : 0; // before this no row sees anything
+            auto look_up = [&](int i) { // page of this lane's box of unit i, -1: nothing to fetch
+                const int key = w.keys.x + (w.ub + i) * BK + box * box_rows;
+                return i < w.take && box < boxes && key < w.keys.y && key + box_rows > seen ? kq_page_of(a.c, w.s, key) : -1;
+            };
+            int id = look_up(0);
+            for (int i = 0; i < w.take; i++) {
+                const int key = w.keys.x + (w.ub + i) * BK + box * box_rows, place = key % a.c.page, next = look_up(i + 1);
+                for (int kv = 0; kv < 2; kv++, tile_n++) {
+                    if constexpr (F8) {
+                        uint64_t &full = sh.raw_full[tile_n % NR];
+                        wait(sh.raw_empty[tile_n % NR], ((tile_n / NR) & 1) ^ 1, 7);
+                        const uint32_t n = __popc(__ballot_sync(0xffffffffu, id >= 0)), bytes = box_rows * HD;
+                        if (lane == 0) expect(smem_u32(&full), *abort ? 0 : n * bytes);
+                        __syncwarp();
+                        if (id >= 0 && !*abort)
+                            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                             smem_u32(sm + L::RAWS + (tile_n % NR) * L::RAW + box * bytes)),
+                                         "l"((kv ? a.c.v : a.c.k) + (int64_t)id * a.c.page_bytes + ((int64_t)w.kh * a.c.page + place) * HD), "r"(bytes), "r"(smem_u32(&full))
+                                         : "memory");
+                    } else {
+                        uint64_t &full = sh.full[tile_n % NS];
+                        wait(sh.empty[tile_n % NS], ((tile_n / NS) & 1) ^ 1, 7);
+                        if (lane == 0) expect(smem_u32(&full), *abort ? 0 : L::TILE);
+                        __syncwarp();
+                        if (box < boxes && !*abort) // a page that is not there comes as zeros: its coordinate is past the end
+                            asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                                             smem_u32(sm + L::RING + (tile_n % NS) * L::TILE + half * HALF + box * box_rows * 128)),
+                                         "l"(kv ? &vmap : &kmap), "r"(64 * half), "r"(w.kh * a.c.page + place), "r"(id >= 0 ? id : (int)a.c.n_pages), "r"(smem_u32(&full))
+                                         : "memory");
+                    }
+                    __syncwarp();
+                }
+                id = next;
+            }
+            w.done();
+        }
+        if (*abort && lane == 0) // what is in flight must land before the CTA goes away
+            for (int i = 0; i < (F8 ? NR : NS); i++) {
+                uint64_t &b = F8 ? sh.raw_full[i] : sh.full[i];
+                kq_mbar_wait(smem_u32(&b), 0u, KQ_WAIT_LIMIT_NS);
+                kq_mbar_wait(smem_u32(&b), 1u, KQ_WAIT_LIMIT_NS);
+            }
+        __syncwarp();
+    } else if (F8 && warp >= 12) {
+        // ---------------------------------------------------------------- e4m3 rows to the f16 tile: a thread per position
+        const int c = tid - 384;
+        uint32_t tile_n = 0;
+        while (w.next(a)) {
+            const int seen = a.window > 0 ? max(0, w.sq.pos(w.tile * R / a.G) - a.window + 1) : 0;
+            auto look_up = [&](int i) {
+                const int key = w.keys.x + (w.ub + i) * BK + c;
+                return i < w.take && key < w.keys.y && key >= seen ? kq_page_of(a.c, w.s, key) : -1;
+            };
+            auto scales = [&](int i, int id) { // of the position's block
+                if (id < 0) return make_float2(0.f, 0.f);
+                const int64_t at = ((int64_t)id * a.c.n_kv + w.kh) * bpp + (w.keys.x + (w.ub + i) * BK + c) % a.c.page / KQ_PAGE_BLOCK;
+                return make_float2(a.c.ks[at], a.c.vs[at]);
+            };
+            int id = look_up(0), id1 = look_up(1); // pages two units ahead, scales one: their loads are under way while a unit is converted
+            float2 sc = scales(0, id);
+            for (int i = 0; i < w.take; i++) {
+                const int id2 = look_up(i + 2);
+                const float2 sc1 = scales(i + 1, id1);
+#pragma unroll 1
+                for (int kv = 0; kv < 2; kv++, tile_n++) {
+                    constexpr int NC = HD / 16; // 16-byte chunks of a raw row; taken in an order that keeps eight rows off each other's banks
+                    uint4 raw[NC];
+                    wait(sh.raw_full[tile_n % NR], (tile_n / NR) & 1, 8);
+                    const uint8_t *src = sm + L::RAWS + (tile_n % NR) * L::RAW + c * HD;
+#pragma unroll
+                    for (int j = 0; j < NC; j++) raw[j] = id >= 0 ? *reinterpret_cast<const uint4 *>(src + ((j + c) % NC) * 16) : make_uint4(0, 0, 0, 0);
+                    arrive(smem_u32(&sh.raw_empty[tile_n % NR]));
+                    const __half2 s = __float2half2_rn(kv ? sc.y : sc.x);
+                    wait(sh.empty[tile_n % NS], ((tile_n / NS) & 1) ^ 1, 9);
+                    uint8_t *dst = sm + L::RING + (tile_n % NS) * L::TILE + c * 128;
+#pragma unroll
+                    for (int j = 0; j < NC; j++) {
+                        const int o = 2 * ((j + c) % NC); // the first of two chunks of 8 dimensions
+                        uint8_t *d = dst + (o >> 3) * HALF;
+                        *reinterpret_cast<uint4 *>(d + (((o & 7) ^ (c & 7)) << 4)) = decode8(raw[j].x, raw[j].y, s);
+                        *reinterpret_cast<uint4 *>(d + ((((o & 7) + 1) ^ (c & 7)) << 4)) = decode8(raw[j].z, raw[j].w, s);
+                    }
+                    fence_async();
+                    arrive(smem_u32(&sh.full[tile_n % NS]));
+                }
+                id = id1;
+                id1 = id2;
+                sc = sc1;
+            }
+            w.done();
+        }
+    } else if (warp < 8) {
+        // ---------------------------------------------------------------- queries, softmax, results: a thread per row
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + COL_S + 128 * half, to = tl + COL_O + 128 * half;
+        uint32_t pieces = 0, units = 0;
+        while (w.next(a)) {
+            const int row0 = w.tile * R + 128 * half; // of this half, within the sequence and KV head
+            // ---- queries: a warp's 32 rows one after another, four rows' loads together; rows of one token share its angles
+            constexpr int P = HD / 64;
+            const bool split = a.turns.on && a.turns.neox;
+            int tok_cs = -1;
+            float2 cs[P];
+#pragma unroll
+            for (int u = 0; u < P; u++) cs[u] = make_float2(1.f, 0.f);
+            // the lane's pairs are P lane + u: dimensions (pair, pair + HD / 2) or (2 pair, 2 pair + 1)
+            for (int rb = 0; rb < 32; rb += 4) {
+                float x[4][P][2];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int rr = row0 + (warp & 3) * 32 + rb + k, tok = rr / a.G;
+#pragma unroll
+                    for (int u = 0; u < P; u++) x[k][u][0] = x[k][u][1] = 0.f;
+                    if (tok >= w.sq.t) continue;
+                    const int64_t at = (int64_t)(w.sq.row0 + tok) * a.q_stride + (int64_t)(w.kh * a.G + rr % a.G) * HD;
+                    if (split && P == 2) {
+                        const float2 v0 = kq_ld2_type(a.type, a.q, at + 2 * lane), v1 = kq_ld2_type(a.type, a.q, at + HD / 2 + 2 * lane);
+                        x[k][0][0] = v0.x, x[k][P - 1][0] = v0.y, x[k][0][1] = v1.x, x[k][P - 1][1] = v1.y;
+                    } else if (split) {
+                        x[k][0][0] = kq_ld1_type(a.type, a.q, at + lane);
+                        x[k][0][1] = kq_ld1_type(a.type, a.q, at + HD / 2 + lane);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < P; u++) {
+                            const float2 v = kq_ld2_type(a.type, a.q, at + 2 * (P * lane + u));
+                            x[k][u][0] = v.x, x[k][u][1] = v.y;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int r = (warp & 3) * 32 + rb + k, rr = row0 + r, tok = rr / a.G;
+                    if (a.turns.on && tok != tok_cs && tok < w.sq.t) {
+                        tok_cs = tok;
+#pragma unroll
+                        for (int u = 0; u < P; u++) cs[u] = kq_turn(a.turns.f[P * lane + u], w.sq.pos(tok));
+                    }
+                    float amax = 0.f;
+#pragma unroll
+                    for (int u = 0; u < P; u++) {
+                        const float v0 = x[k][u][0], v1 = x[k][u][1];
+                        x[k][u][0] = v0 * cs[u].x - v1 * cs[u].y;
+                        x[k][u][1] = v0 * cs[u].y + v1 * cs[u].x;
+                        amax = fmaxf(amax, fmaxf(fabsf(x[k][u][0]), fabsf(x[k][u][1])));
+                    }
+                    amax = kq_warp_max(amax);
+                    const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 252u);
+                    const float f = amax > 0.f ? __uint_as_float((254u - e) << 23) : 1.f;
+                    if (lane == 0) sh.crow[128 * half + r] = fmaxf(amax > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2, 1.2e-38f); // not 0: a hidden score times it is -inf
+                    auto put = [&](int d, float v0, float v1, bool two) { // dimension d (and d + 1)
+#pragma unroll
+                        for (int p = 0; p < QS; p++) {
+                            uint8_t *at = sm + (2 * p + half) * L::TILE + (d >> 6) * HALF + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2;
+                            const uint32_t hi = h2(v0, v1), v = p ? h2_low(v0, v1, hi) : hi;
+                            if (two) *reinterpret_cast<uint32_t *>(at) = v;
+                            else *reinterpret_cast<uint16_t *>(at) = (uint16_t)v;
+                        }
+                    };
+                    if (split && P == 2) {
+                        put(2 * lane, x[k][0][0] * f, x[k][P - 1][0] * f, true);
+                        put(HD / 2 + 2 * lane, x[k][0][1] * f, x[k][P - 1][1] * f, true);
+                    } else if (split) {
+                        put(lane, x[k][0][0] * f, 0.f, false);
+                        put(HD / 2 + lane, x[k][0][1] * f, 0.f, false);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < P; u++) put(2 * (P * lane + u), x[k][u][0] * f, x[k][u][1] * f, true);
+                    }
+                }
+            }
+            fence_async();
+            arrive(smem_u32(&sh.q_ready));
+            __syncwarp();
+            const float crow = sh.crow[128 * half + row];
+            const int my_tok = min((row0 + row) / a.G, w.sq.t - 1), lim = w.sq.p0 < 0 ? -1 : w.sq.pos(my_tok); // last position this row sees
+            const int lim_lo = w.sq.pos(min(row0 / a.G, w.sq.t - 1)), lim_hi = w.sq.pos(min((row0 + 127) / a.G, w.sq.t - 1)); // of the half's rows
+            const int seen = a.window > 0 ? max(0, w.sq.pos(w.tile * R / a.G) - a.window + 1) : 0;
+            auto look_up = [&](int i) { // is the lane's block (of 32 from unit i on) there
+                const int key = w.keys.x + (w.ub + i) * BK + KQ_PAGE_BLOCK * lane;
+                return key < w.keys.y ? kq_page_of(a.c, w.s, key) : -1;
+            };
+            uint32_t there = 0;
+            int ahead = look_up(0);
+            float m = -INFINITY, l = 0.f;
+            for (int i = 0; i < w.take; i++, units++) {
+                if ((i & 3) == 0) {
+                    there = __ballot_sync(0xffffffffu, ahead >= 0);
+                    ahead = look_up(i + 4);
+                }
+                const uint32_t blocks = (there >> (8 * (i & 3))) & 0xff;
+                const int key0 = w.keys.x + (w.ub + i) * BK;
+                wait(sh.s_ready[half], units & 1, 10);
+                after_sync();
+                // the scores are read twice, 32 at a time (the maximum, then the probabilities): a row of 128 would not fit next to the rest
+                const bool masked = blocks != 0xff || key0 + BK - 1 > lim_lo || (a.window > 0 && key0 <= lim_hi - a.window);
+                const int last = lim - key0, first = a.window > 0 ? last - a.window + 1 : -0x7fffffff;
+                auto mask = [&](uint32_t *s, int c) {
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (32 * c + j > last || 32 * c + j < first || !(blocks >> ((32 * c + j) >> 4) & 1)) s[j] = 0xff800000u; // -inf
+                };
+                uint32_t s[2][32];
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_ld32(ts, s[0]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    tmem_ld_wait();
+                    tmem_ld32(ts + 32 * ((c + 1) & 3), s[(c + 1) & 1]); // the last one begins the second reading
+                    if (masked) mask(s[c & 1], c);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[c & 1][j]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * crow;
+                const bool grown = top > m + 8.f || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float mn = grown ? fmaxf(m, top) : m, alpha = mn == m ? 1.f : ex2(m - mn);
+                    m = mn;
+                    if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) { // S of this tile was issued behind the product before: O is at rest
+                        l *= alpha;
+#pragma unroll
+                        for (int k = 0; k < HD / 32; k++) {
+                            uint32_t o[32];
+                            tmem_ld32(to + 32 * k, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+                            if (!*abort) tmem_st32(to + 32 * k, o);
+                        }
+                    }
+                }
+                const float sub = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t lo_even[PS == 2 ? 16 : 1];
+                // a chunk's probabilities go over scores that have been read: those of keys 0 .. 63 to columns 0 .. 31 (second parts 32 .. 63) ...
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    tmem_ld_wait();
+                    if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[(c + 1) & 1]);
+                    uint32_t(&x)[32] = s[c & 1];
+                    if (masked) mask(x, c);
+                    uint32_t hi[16], lo[PS == 2 ? 16 : 1];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float p0 = ex2(fmaf(__uint_as_float(x[2 * j]), crow, -sub)), p1 = ex2(fmaf(__uint_as_float(x[2 * j + 1]), crow, -sub));
+                        sum[j & 3] += p0 + p1;
+                        hi[j] = h2(p0, p1);
+                        if (PS == 2) lo[PS == 2 ? j : 0] = h2_low(p0, p1, hi[j]);
+                    }
+                    if (PS == 2 && (c & 1) == 0) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) lo_even[PS == 2 ? j : 0] = lo[PS == 2 ? j : 0];
+                    }
+                    if (!*abort) {
+                        tmem_st16(ts + 64 * (c >> 1) + 16 * (c & 1), hi);
+                        if (PS == 2 && (c & 1)) { // columns 32 .. 63 of the half are free once its second chunk has been read
+                            tmem_st16(ts + 64 * (c >> 1) + 32, lo_even);
+                            tmem_st16(ts + 64 * (c >> 1) + 48, lo);
+                        }
+                    }
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (!F8 && half == 0 && (key0 + BK > w.keys.y || key0 < seen)) {
+                    // a value that no row sees may hold anything: it must not meet a probability of 0
+                    const uint32_t v = 2 * units + 1;
+                    wait(sh.full[v % NS], (v / NS) & 1, 11);
+                    if (key0 + row >= w.keys.y || key0 + row < seen) {
+                        uint8_t *d = sm + L::RING + (v % NS) * L::TILE + row * 128;
+#pragma unroll
+                        for (int j = 0; j < HD / 8; j++) *reinterpret_cast<uint4 *>(d + (j >> 3) * HALF + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_async();
+                }
+                tmem_st_wait();
+                before_sync();
+                arrive(smem_u32(&sh.p_ready[half]));
+            }
+            // ---- results
+            wait(sh.o_done, pieces & 1, 12);
+            after_sync();
+            const bool whole = w.ub == 0 && w.take == w.n_units, ok = (row0 + row) / a.G < w.sq.t && !*abort;
+            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            const int64_t at = whole ? (int64_t)(w.sq.row0 + my_tok) * a.out_stride + (int64_t)(w.kh * a.G + (row0 + row) % a.G) * HD
+                                     : (int64_t)(2 * blockIdx.x + (w.ub == 0 ? 1 : 0)) * R * (HD + 2) + (int64_t)(128 * half + row) * HD;
+#pragma unroll
+            for (int k = 0; k < HD / 32; k++) {
+                uint32_t o[32];
+                tmem_ld32(to + 32 * k, o);
+                tmem_ld_wait();
+                if (!ok) continue;
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int x = 0; x < 8; x++) v[x] = l == 0.f ? 0.f : __uint_as_float(o[j + x]) * inv; // nothing seen: O is 0 by zeros
+                    if (!whole || a.type == B200_TYPE_F32) {
+                        float *p = (whole ? (float *)a.out : a.part) + at + 32 * k + j;
+                        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        uint4 u;
+                        if (a.type == B200_TYPE_F16) u = make_uint4(h2(v[0], v[1]), h2(v[2], v[3]), h2(v[4], v[5]), h2(v[6], v[7]));
+                        else {
+                            const __nv_bfloat162 b[4] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3]), __floats2bfloat162_rn(v[4], v[5]),
+                                                         __floats2bfloat162_rn(v[6], v[7])};
+                            u = *reinterpret_cast<const uint4 *>(b);
+                        }
+                        *reinterpret_cast<uint4 *>((uint16_t *)a.out + at + 32 * k + j) = u;
+                    }
+                }
+            }
+            if (!whole && ok) {
+                float *ml = a.part + (int64_t)(2 * blockIdx.x + (w.ub == 0 ? 1 : 0)) * R * (HD + 2) + (int64_t)R * HD + 2 * (128 * half + row);
+                *reinterpret_cast<float2 *>(ml) = make_float2(m, l);
+            }
+            if (tid == 0 && w.ub == 0 && !whole) meta = make_int4(1 + (int)((w.n_units - w.take + (run.u1 - run.u0) - 1) / (run.u1 - run.u0)), w.s, w.kh, w.tile);
+            before_sync();
+            pieces++;
+            w.done();
+        }
+        if (tid == 0) a.meta[blockIdx.x] = meta;
+    }
+    before_sync();
+    __syncthreads();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// joins the pieces of a split item: a warp per row, lanes the dimensions; grid (CTAs of the attention kernel, R / 16)
+template <int HD> __global__ void __launch_bounds__(256) pages_join_kernel(const __grid_constant__ KqAttnArgs a) {
+    KQ_PDL_ENTER();
+    const int4 meta = a.meta[blockIdx.x];
+    if (meta.x == 0) return;
+    const KqSeq sq = kq_seq(a, meta.y);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int N = HD / 64;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int r = blockIdx.y * 16 + 2 * warp + k, rr = meta.w * R + r, tok = rr / a.G;
+        if (tok >= sq.t) continue;
+        float m = -INFINITY, l = 0.f;
+        float2 o[N];
+#pragma unroll
+        for (int u = 0; u < N; u++) o[u] = make_float2(0.f, 0.f);
+        for (int i0 = 0; i0 < meta.x; i0 += 4) {
+            float2 ml[4], v[4][N];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int i = i0 + j;
+                ml[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int u = 0; u < N; u++) v[j][u] = make_float2(0.f, 0.f);
+                if (i < meta.x) { // piece 0 is slot 2 b + 1, piece i slot 2 (b + i)
+                    const float *p = a.part + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * R * (HD + 2);
+                    ml[j] = *reinterpret_cast<const float2 *>(p + R * HD + 2 * r);
+#pragma unroll
+                    for (int u = 0; u < N; u++) v[j][u] = *reinterpret_cast<const float2 *>(p + r * HD + 2 * (lane + 32 * u));
+                }
+            }
+            const float mn = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), sub = mn == -INFINITY ? 0.f : mn;
+            const float f0 = ex2(m - sub);
+            l *= f0;
+#pragma unroll
+            for (int u = 0; u < N; u++) o[u].x *= f0, o[u].y *= f0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float f = ex2(ml[j].x - sub);
+                l += f * ml[j].y;
+#pragma unroll
+                for (int u = 0; u < N; u++) o[u].x += f * v[j][u].x, o[u].y += f * v[j][u].y;
+            }
+            m = mn;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            kq_st2_type(a.type, a.out, (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(meta.z * a.G + rr % a.G) * HD + 2 * (lane + 32 * u), o[u].x * inv, o[u].y * inv);
+    }
+}
+
+template <int HD, bool F8, int QS, int PS> b200_status launch(const KqAttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int box_rows, int ctas, cudaStream_t st) {
+    static bool attr[64];
+    int dev = 0;
+    KQ_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr[dev]) {
+        KQ_CUDA(cudaFuncSetAttribute(pages_prompt_kernel<HD, F8, QS, PS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD, F8, QS>::TOTAL));
+        if (dev >= 0 && dev < 64) attr[dev] = true;
+    }
+    kq_launch(pages_prompt_kernel<HD, F8, QS, PS>, ctas, F8 ? 512 : 384, Layout<HD, F8, QS>::TOTAL, st, a, k, v, box_rows);
+    KQ_COUNT_LAUNCH();
+    KQ_LAUNCH_CHECK();
+    return B200_OK;
+}
+template <int HD, bool F8> b200_status launch(const KqAttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int box_rows, int ctas, cudaStream_t st) {
+    if (a.type == B200_TYPE_F32) return launch<HD, F8, 2, 2>(a, k, v, box_rows, ctas, st);
+    if (a.type == B200_TYPE_F16 && a.turns.on) return launch<HD, F8, 2, 1>(a, k, v, box_rows, ctas, st);
+    return launch<HD, F8, 1, 1>(a, k, v, box_rows, ctas, st);
+}
+
+constexpr size_t META_BYTES = 4096;
+
+} // namespace
+
+int kq_pages_error_fetch() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_pages_error, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(g_pages_error, &zero, sizeof(int));
+    return v;
+}
+
+size_t kq_pages_prompt_scratch(int hd) { return META_BYTES + (size_t)kq_sm_count() * 2 * R * (hd + 2) * sizeof(float); }
+
+b200_status kq_pages_prompt(KqAttnArgs a, bool f8, int hd, uint8_t *scratch, cudaStream_t st) {
+    const int ctas = kq_sm_count();
+    KQ_REQUIRE((size_t)ctas * sizeof(int4) <= META_BYTES, "attention_pages: %d multiprocessors", ctas);
+    a.meta = (int4 *)scratch;
+    a.part = (float *)(scratch + META_BYTES);
+    int box_rows = 128; // the largest power of two that divides the page
+    while (a.c.page % box_rows) box_rows /= 2;
+    CUtensorMap maps[2];
+    memset(maps, 0, sizeof(maps));
+    if (!f8)
+        for (int i = 0; i < 2; i++) {
+            const uint64_t dims[3] = {(uint64_t)hd, (uint64_t)a.c.n_kv * a.c.page, (uint64_t)a.c.n_pages}, strides[2] = {(uint64_t)hd * 2, (uint64_t)a.c.page_bytes};
+            const uint32_t box[3] = {64, (uint32_t)box_rows, 1};
+            KQ_TRY(kq_tmap_encode(&maps[i], 2, 3, i ? a.c.v : a.c.k, dims, strides, box, 1));
+        }
+    if (hd == 128) KQ_TRY(f8 ? (launch<128, true>(a, maps[0], maps[1], box_rows, ctas, st)) : (launch<128, false>(a, maps[0], maps[1], box_rows, ctas, st)));
+    else KQ_TRY(f8 ? (launch<64, true>(a, maps[0], maps[1], box_rows, ctas, st)) : (launch<64, false>(a, maps[0], maps[1], box_rows, ctas, st)));
+    kq_launch(hd == 128 ? pages_join_kernel<128> : pages_join_kernel<64>, dim3((unsigned)ctas, R / 16), 256, 0, st, a);
+    KQ_COUNT_LAUNCH();
+    KQ_LAUNCH_CHECK();
+    return B200_OK;
+}

@@ -33,14 +33,15 @@ __device__ __forceinline__ KqSeq kq_seq(const KqAttnArgs &a, int s) {
     const int64_t n = (int64_t)(r.y - r.x) * a.G;
     return KqSeq{n >= a.t_lo && n <= a.t_hi ? r.y - r.x : 0, a.b.pos0[s], r.x};
 }
-template <int R> __device__ __forceinline__ int kq_tiles(const KqAttnArgs &a, int t) { return (int)(((int64_t)t * a.G + R - 1) / R); }
-// positions [x, y) that some row of the tile sees; x is a multiple of 16
+template <int R> __device__ __forceinline__ int kq_tiles(const KqAttnArgs &a, int t) { return (t * a.G + R - 1) / R; }
+// positions [x, y) that some row of the tile sees, x rounded down to a block, or for tiles of 256 rows to a whole unit
 template <int R> __device__ __forceinline__ int2 kq_tile_keys(const KqAttnArgs &a, const KqSeq &q, int tile) {
-    const int first = (int)((int64_t)tile * R / a.G), last = (int)min((int64_t)q.t - 1, ((int64_t)tile * R + R - 1) / a.G);
+    constexpr int A = R >= 128 ? 128 : KQ_PAGE_BLOCK;
+    const int first = tile * R / a.G, last = min(q.t - 1, (tile * R + R - 1) / a.G); // rows x heads stay below 2^30
     const int64_t cap = (int64_t)a.c.table_len * a.c.page;
     const int hi = q.p0 < 0 ? 0 : (int)min((int64_t)q.p0 + last + 1, cap);
-    const int lo = a.window > 0 ? (int)max((int64_t)0, (int64_t)q.p0 + first - a.window + 1) & ~(KQ_PAGE_BLOCK - 1) : 0;
-    return make_int2(min(lo, hi & ~(KQ_PAGE_BLOCK - 1)), hi);
+    const int lo = a.window > 0 ? (int)max((int64_t)0, (int64_t)q.p0 + first - a.window + 1) & ~(A - 1) : 0;
+    return make_int2(min(lo, hi & ~(A - 1)), hi);
 }
 template <int U> __device__ __forceinline__ int kq_units(int2 keys) { return max(1, (keys.y - keys.x + U - 1) / U); }
 template <int R, int U> __device__ __forceinline__ long long kq_head_units(const KqAttnArgs &a, const KqSeq &q) {
@@ -103,3 +104,6 @@ b200_status kq_pages_combine(const KqAttnArgs &a, int hd, int R, int ctas, cudaS
 // sequences of few rows (any number is right), and its workspace
 size_t kq_pages_decode_scratch(int hd);
 b200_status kq_pages_decode(KqAttnArgs a, bool f8, int hd, int64_t most, uint8_t *scratch, cudaStream_t st);
+// sequences of many rows
+size_t kq_pages_prompt_scratch(int hd);
+b200_status kq_pages_prompt(KqAttnArgs a, bool f8, int hd, uint8_t *scratch, cudaStream_t st);

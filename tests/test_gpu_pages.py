@@ -195,6 +195,36 @@ def test_ragged(cache, hd, window, neox):
         assert (got[:2] == 7).all() and (got[b.rows:] == 7).all()  # rows nobody owns
 
 
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1, 64), (5, 1, 128), (8, 2, 128), (14, 2, 64)])
+def test_prompts(cache, dtype, shape):
+    """one sequence, from nothing and behind a long past: one and many tiles of rows, tiles of keys that end anywhere"""
+    n_head, n_kv, hd = shape
+    for new, past, page in ((130, 0, 16), (67, 61, 48), (300, 1000, 128), (513, 129, 64)):
+        c, b = Cache(1, new + past, page, n_kv, hd, cache, seed=10), Batch([new], [past])
+        fill(c, [past], 110, 1e6, 1)
+        q = rows(33, new, n_head, hd, dtype)
+        c.append(rows(34, new, n_kv, hd, dtype), rows(35, new, n_kv, hd, dtype), b, 1e6, 1)
+        close(c.attend(q, b, 1e6, 1), attention(c, q, b, 1e6, 1), dtype)
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+@pytest.mark.parametrize("window", [0, 64, 333])
+def test_prompts_and_steps_in_one_call(cache, window):
+    new, past = [200, 1, 0, 3, 90, 1, 400, 65], [10, 700, 5, 129, 0, 0, 600, 128]
+    n_head, n_kv, hd = 10, 2, 128
+    c, b = Cache(8, 1000, 32, n_kv, hd, cache, seed=11), Batch(new, past, first=1)
+    fill(c, past, 120, 1e4, 0)
+    q = rows(36, b.rows, n_head, hd)
+    c.append(rows(37, b.rows, n_kv, hd), rows(38, b.rows, n_kv, hd), b, 1e4, 0)
+    out = torch.full((b.rows + 2, n_head, hd), 7.0, device="cuda")
+    got = c.attend(torch.cat((q, q[:2])), b, 1e4, 0, window=window, out=out)
+    close(got[1:b.rows], attention(c, q, b, 1e4, 0, window)[1:], torch.float32)
+    assert (got[0] == 7).all() and (got[b.rows:] == 7).all()
+    assert torch.equal(c.attend(torch.cat((q, q[:2])), b, 1e4, 0, window=window, out=torch.full_like(out, 7.0)), got)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_e4m3_pages_give_what_the_f16_pages_of_their_values_give(dtype):
     c = Cache(3, 700, 32, 2, 128, F8, seed=7)
