@@ -47,6 +47,8 @@ __device__ __forceinline__ float2 kq_turn(double f, int pos) {
     sincospif(2.f * tf, &s, &c);
     return make_float2(fmaf(-s, d, c), fmaf(c, d, s));
 }
+// the same out of line, where it would be inlined many times over
+static __device__ __noinline__ float2 kq_turn_call(double f, int pos) { return kq_turn(f, pos); }
 // first and past-the-last row of sequence s, inside the call's rows whatever row_start holds
 __device__ __forceinline__ int2 kq_seq_rows(const KqBatch &b, int s) {
     const int lo = min(max(b.row_start[s], 0), b.rows), hi = min(max(b.row_start[s + 1], lo), b.rows);
@@ -69,13 +71,14 @@ __device__ __forceinline__ uint32_t kq_e4m3x2_h2(uint16_t v) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
     return r;
 }
-// activations of two neighbouring elements as f32 and back
+// activations as f32
 template <typename T> __device__ __forceinline__ float2 kq_ld2(const T *p);
 template <> __device__ __forceinline__ float2 kq_ld2<float>(const float *p) { return *reinterpret_cast<const float2 *>(p); }
 template <> __device__ __forceinline__ float2 kq_ld2<__half>(const __half *p) { return __half22float2(*reinterpret_cast<const __half2 *>(p)); }
 template <> __device__ __forceinline__ float2 kq_ld2<__nv_bfloat16>(const __nv_bfloat16 *p) {
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(p));
 }
+template <typename T> __device__ __forceinline__ float kq_ld1(const T *p) { return (float)*p; }
 __device__ __forceinline__ float2 kq_ld2_type(uint32_t type, const void *p, int64_t at) {
     return type == B200_TYPE_F32 ? kq_ld2((const float *)p + at) : type == B200_TYPE_F16 ? kq_ld2((const __half *)p + at) : kq_ld2((const __nv_bfloat16 *)p + at);
 }

@@ -1,13 +1,16 @@
 // Attention of a few new rows per sequence over paged keys and values (b200_attention_pages): decode steps and drafts.
 //
-// A warp takes 16 positions (f16) or 32 (e4m3) of an item at a time straight from the pages into registers, as the fragments
-// of mma.m16n8k16: nothing goes through shared memory.  That works because the order of a product's inner index is free: a thread
-// reads 16 bytes of a key, which are the dimensions that its lane holds in consecutive steps of Q K^T, and Q is laid out to match; of the
-// values it reads 16 bytes of four keys and pairs them up by byte permutes into the rows of V^T.  e4m3 codes become f16 in
-// registers (K's scale goes onto the score, V's onto the value, both exact powers of two).  Scores are Q K^T with the item's rows as
-// the 16 rows of the tile; the probabilities are then already the B operand of O^T = V^T P^T.  Softmax in base 2, statistics in 32 bits.
+// A warp takes 16 positions (f16) or 32 (e4m3) of an item at a time through its own ring in shared memory, filled by 16-byte
+// asynchronous copies (what no row sees, or is not there, arrives as zeros), so that loads stay in flight under the arithmetic and no warp waits for another.
+// From there the fragments of mma.m16n8k16 are 16-byte reads: the order of a product's inner index is free, so the 16 bytes that a thread reads of a
+// key are the dimensions that its lane holds in consecutive steps of Q K^T, and Q is laid out to match; of the values it
+// reads 16 bytes of four keys and pairs them up by byte permutes into the rows of V^T.  16-byte chunks are stored at chunk ^ (row % 8), which keeps both
+// kinds of read off each other's banks.  e4m3 codes become f16 in registers (K's scale goes onto the score, V's onto the value, both
+// exact powers of two).  Scores are Q K^T with the item's rows as the 16 rows of the tile; the probabilities are then already the
+// B operand of O^T = V^T P^T.  Softmax in base 2, statistics in 32 bits.
 // A query row enters divided by the power of two that brings its largest element to [1, 2), so f16 neither overflows nor loses small
-// rows; f32 rows go in as two f16 parts (22 bits), and so do their probabilities.
+// rows; f32 and f16 rows go in as two f16 parts (rotation makes an f16 query longer than f16), and so do their probabilities; the tensor cores
+// cut their sums off instead of rounding them, so those of one step (16 or 32 keys) are added to the row in 32-bit registers.
 //
 // Bound by HBM: a position costs 2 hd codes per KV head and is read once.  The units of all items are shared out evenly
 // (kq_pages_sched.cuh), the four warps of a CTA take neighbouring positions and join their rows through shared memory at an item's end.
@@ -16,22 +19,21 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
 constexpr int NT = 128, NW = NT / 32;
 constexpr int MAX_CTAS_PER_SM = 4;
 
-__device__ __forceinline__ uint4 ld16(const uint8_t *p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes to shared memory, zeros where `there` is false (nothing is read then)
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ uint4 ld8(const uint8_t *p) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -56,29 +58,49 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// HT: tiles of 8 rows (1 or 2); SPLIT: queries and probabilities in two f16 parts
-template <int HD, bool F8, int HT, bool SPLIT>
-__global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const __grid_constant__ KqAttnArgs a) {
-    constexpr int R = 8 * HT, ES = F8 ? 1 : 2, NG = F8 ? 2 : 1, KT = 16 * NG, U = NW * KT; // groups of 16 positions of a warp's step; positions of a unit
-    constexpr int KL = HD * ES / 64, VL = (HD * ES + 127) / 128;                           // 16-byte loads of a key and of a value
-    constexpr int KS = HD / 16, MT = HD / 16;                                              // steps of Q K^T, tiles of 16 dimensions of O^T
+template <int HD, bool F8, int HT> struct Shape {
+    static constexpr int R = 8 * HT, ES = F8 ? 1 : 2, ROW = HD * ES, NG = F8 ? 2 : 1, KT = 16 * NG; // groups of 16 positions of a warp's step
+    static constexpr int STEP = 2 * KT * ROW;                                                       // keys, then values
+    static constexpr int NST = STEP == 8192 ? (HT == 1 ? 2 : 3) : 4;                                // ring stages of a warp
+    static constexpr int CTAS = HT == 1 ? 3 : 2;                                                    // per SM
+    static constexpr int SMEM = NW * NST * STEP;
+    static_assert(NST * STEP >= R * HD * 4, "a warp's rows fit into its ring");
+};
+// place of 16-byte chunk c of row r
+template <int ROW> __device__ __forceinline__ int place(int r, int c) { return r * ROW + ((c ^ (ROW >= 128 ? r & 7 : (r >> 1) & 3)) << 4); }
+
+// HT: tiles of 8 rows (1 or 2); T: the activations' type, all but bf16 (whose results have 8 bits) with queries and probabilities in two f16 parts
+template <int HD, bool F8, int HT, typename T>
+__global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kernel(const __grid_constant__ KqAttnArgs a) {
+    using S = Shape<HD, F8, HT>;
+    constexpr bool SPLIT = !std::is_same<T, __nv_bfloat16>::value;
+    constexpr int R = S::R, ROW = S::ROW, NG = S::NG, KT = S::KT, U = NW * KT, NST = S::NST;
+    constexpr int KL = ROW / 64, VL = (ROW + 127) / 128; // 16-byte reads of a key and of a value
+    constexpr int KS = HD / 16, MT = HD / 16;            // steps of Q K^T, tiles of 16 dimensions of O^T
     constexpr int QP = HD + 4;
+    extern __shared__ __align__(128) uint8_t ring_s[];
     __shared__ __align__(16) float q_s[R][QP];
     __shared__ float c_s[R];
-    __shared__ __align__(16) float o_s[NW][R][HD];
+    __shared__ float sc_s[NW][NST][4];  // scales of the step's groups: keys, values
+    __shared__ int have_s[NW][NST];     // which of them are there
     __shared__ float m_s[NW][R], l_s[NW][R];
+    __shared__ double turns_s[HD / 2]; // a lane's own entry is no broadcast: not from the constant bank
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    if (tid < HD / 2) turns_s[tid] = a.turns.f[tid];
+    uint8_t *ring = ring_s + warp * (NST * S::STEP);
+    const uint32_t ring_u = smem_u32(ring);
+    auto o_at = [&](int w) { return reinterpret_cast<float (*)[HD]>(ring_s + w * (NST * S::STEP)); }; // a warp's rows, once its ring is done
     KQ_PDL_ENTER();
     KqRun run = kq_find_run<R, U, NT>(a);
-    int4 meta = make_int4(0, 0, 0, 0);
+    int4 meta = make_int4(0, 0, 0, 0), meta2 = meta;
     long long u = run.u0;
     for (int s = run.s; u < run.u1 && s < a.b.n_seq; s++, run.off = 0) {
         const KqSeq sq = kq_seq(a, s);
         if (sq.t == 0) continue;
         const int tiles = kq_tiles<R>(a, sq.t);
-        const long long per_head = kq_head_units<R, U>(a, sq);
-        int kh = (int)(run.off / per_head), tile = 0;
-        long long uo = run.off % per_head;
+        const long long per_head = run.off ? run.per_head : 1; // only the sequence that the run begins in begins inside
+        int kh = (int)kq_div(run.off, per_head), tile = 0;
+        long long uo = run.off - kh * per_head;
         while (tile < tiles) { // the tile that the run begins in
             const int n = kq_units<U>(kq_tile_keys<R>(a, sq, tile));
             if (uo < n) break;
@@ -90,37 +112,88 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                 const int2 keys = kq_tile_keys<R>(a, sq, tile);
                 const int n_units = kq_units<U>(keys), take = (int)min((long long)n_units - uo, run.u1 - u), ub = (int)uo;
                 u += take;
+                __syncthreads(); // the item before has been joined
+                const int bpp = a.c.page / KQ_PAGE_BLOCK;
+                const int64_t head_off = (int64_t)kh * a.c.page * ROW;
+                const int see_all = sq.pos(tile * R / a.G); // positions up to here every row sees ...
+                const int see_from = a.window > 0 ? sq.pos(min((tile * R + R - 1) / a.G, sq.t - 1)) - a.window + 1 : 0; // ... from here on
+                const int first_seen = a.window > 0 ? max(0, see_all - a.window + 1) : 0;                               // before this one none does
+                // ---- asks for the positions of step i
+                int pg[NG], inb[NG]; // page and block in it of this lane's step of the next 32
+                auto ask = [&](int i) {
+                    if (i >= take) {
+                        copies_commit();
+                        return;
+                    }
+                    if ((i & 31) == 0) {
+#pragma unroll
+                        for (int n = 0; n < NG; n++) {
+                            const int key = keys.x + (ub + i + lane) * U + warp * KT + 16 * n;
+                            pg[n] = -1;
+                            inb[n] = 0;
+                            if (i + lane < take && key < keys.y) {
+                                const int blk = key / KQ_PAGE_BLOCK, pi = blk / bpp;
+                                inb[n] = blk - pi * bpp;
+                                const int id = pi < a.c.table_len ? a.c.table[(int64_t)s * a.c.table_stride + pi] : -1;
+                                pg[n] = id >= 0 && id < a.c.n_pages ? id : -1;
+                            }
+                        }
+                    }
+                    const int st = i % NST, key0 = keys.x + (ub + i) * U + warp * KT;
+                    int have = 0;
+#pragma unroll
+                    for (int n = 0; n < NG; n++) {
+                        const int p = __shfl_sync(0xffffffffu, pg[n], i & 31), ib = __shfl_sync(0xffffffffu, inb[n], i & 31);
+                        const int64_t off = (int64_t)max(p, 0) * a.c.page_bytes + head_off + (int64_t)ib * (KQ_PAGE_BLOCK * ROW);
+                        have |= (p >= 0) << n;
+                        constexpr int CH = ROW / 16, PER = 16 * CH / 32; // chunks of a row; copies of a lane
+                        const uint32_t dst = ring_u + st * S::STEP;
+#pragma unroll
+                        for (int j = 0; j < PER; j++) {
+                            const int x = j * 32 + lane, r = x / CH, c = x % CH, key = key0 + 16 * n + r;
+                            const bool there = p >= 0 && key < keys.y && key >= first_seen; // what no row sees may hold anything: it must not meet a probability of 0
+                            copy16(dst + place<ROW>(16 * n + r, c), a.c.k + off + r * ROW + c * 16, there);
+                            copy16(dst + KT * ROW + place<ROW>(16 * n + r, c), a.c.v + off + r * ROW + c * 16, there);
+                        }
+                        if (F8 && p >= 0 && lane < 2)
+                            copy4(smem_u32(&sc_s[warp][st][2 * lane + n]), (lane ? a.c.vs : a.c.ks) + ((int64_t)p * a.c.n_kv + kh) * bpp + ib);
+                    }
+                    if (lane == 0) have_s[warp][st] = have;
+                    copies_commit();
+                };
+                for (int i = 0; i < NST - 1; i++) ask(i);
                 // ---- the item's queries: rotated, normed, in shared memory
-                __syncthreads();
+#pragma unroll 1
                 for (int r = warp; r < R; r += NW) {
-                    const int rr = tile * R + r, tok = rr / a.G, h = kh * a.G + rr % a.G;
+                    const int rr = tile * R + r, tok = rr / a.G, h = kh * a.G + rr - tok * a.G;
                     const bool ok = tok < sq.t;
-                    float amax = 0.f, x[HD / 32];
+                    const T *row = (const T *)a.q + (int64_t)(sq.row0 + (ok ? tok : 0)) * a.q_stride + (int64_t)(ok ? h : 0) * HD;
+                    float x[HD / 32];
 #pragma unroll
                     for (int i = 0; i < HD / 64; i++) {
-                        x[2 * i] = x[2 * i + 1] = 0.f;
-                        if (!ok) continue;
-                        const int pr = lane + 32 * i, d0 = a.turns.neox ? pr : 2 * pr, d1 = a.turns.neox ? pr + HD / 2 : 2 * pr + 1;
-                        const int64_t at = (int64_t)(sq.row0 + tok) * a.q_stride + (int64_t)h * HD;
-                        float v0 = kq_ld1_type(a.type, a.q, at + d0), v1 = kq_ld1_type(a.type, a.q, at + d1);
+                        const int pr = lane + 32 * i;
+                        x[2 * i] = ok ? kq_ld1(row + (a.turns.neox ? pr : 2 * pr)) : 0.f;
+                        x[2 * i + 1] = ok ? kq_ld1(row + (a.turns.neox ? pr + HD / 2 : 2 * pr + 1)) : 0.f;
+                    }
+                    float amax = 0.f;
+#pragma unroll
+                    for (int i = 0; i < HD / 64; i++) {
+                        const float v0 = x[2 * i], v1 = x[2 * i + 1];
                         if (a.turns.on) {
-                            const float2 cs = kq_turn(a.turns.f[pr], sq.pos(tok));
-                            const float w0 = v0 * cs.x - v1 * cs.y;
-                            v1 = v0 * cs.y + v1 * cs.x;
-                            v0 = w0;
+                            const float2 cs = kq_turn_call(turns_s[lane + 32 * i], sq.pos(tok));
+                            x[2 * i] = v0 * cs.x - v1 * cs.y;
+                            x[2 * i + 1] = v0 * cs.y + v1 * cs.x;
                         }
-                        x[2 * i] = v0;
-                        x[2 * i + 1] = v1;
-                        amax = fmaxf(amax, fmaxf(fabsf(v0), fabsf(v1)));
+                        amax = fmaxf(amax, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
                     }
                     amax = kq_warp_max(amax);
                     const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 252u);
                     const float f = amax > 0.f ? __uint_as_float((254u - e) << 23) : 1.f;
 #pragma unroll
                     for (int i = 0; i < HD / 64; i++) {
-                        const int pr = lane + 32 * i, d0 = a.turns.neox ? pr : 2 * pr, d1 = a.turns.neox ? pr + HD / 2 : 2 * pr + 1;
-                        q_s[r][d0] = x[2 * i] * f;
-                        q_s[r][d1] = x[2 * i + 1] * f;
+                        const int pr = lane + 32 * i;
+                        q_s[r][a.turns.neox ? pr : 2 * pr] = x[2 * i] * f;
+                        q_s[r][a.turns.neox ? pr + HD / 2 : 2 * pr + 1] = x[2 * i + 1] * f;
                     }
                     if (lane == 0) c_s[r] = amax > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2;
                 }
@@ -157,69 +230,14 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
 #pragma unroll
                     for (int i = 0; i < MT; i++) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
                 }
-                const int see_all = sq.pos(tile * R / a.G);                                                                    // positions up to here every row sees ...
-                const int see_from = a.window > 0 ? sq.pos(min((tile * R + R - 1) / a.G, sq.t - 1)) - a.window + 1 : 0; // ... from here on
-                const int first_seen = a.window > 0 ? max(0, see_all - a.window + 1) : 0;                // before this one none does
-                const int bpp = a.c.page / KQ_PAGE_BLOCK;
-                const int64_t head_off = (int64_t)kh * a.c.page * HD * ES;
-                int pg[NG], inb[NG]; // page and block in it of this lane's step
                 for (int i = 0; i < take; i++) {
-                    if ((i & 31) == 0) { // a lane looks one of the next 32 steps up
-#pragma unroll
-                        for (int n = 0; n < NG; n++) {
-                            const int key = keys.x + (ub + i + lane) * U + warp * KT + 16 * n;
-                            pg[n] = -1;
-                            inb[n] = 0;
-                            if (i + lane < take && key < keys.y) {
-                                const int blk = key / KQ_PAGE_BLOCK, pi = blk / bpp;
-                                inb[n] = blk - pi * bpp;
-                                const int id = pi < a.c.table_len ? a.c.table[(int64_t)s * a.c.table_stride + pi] : -1;
-                                pg[n] = id >= 0 && id < a.c.n_pages ? id : -1;
-                            }
-                        }
-                    }
-                    const int key0 = keys.x + (ub + i) * U + warp * KT;
+                    copies_wait<NST - 2>();
+                    __syncwarp(); // every lane's copies of step i are in, and every lane is done with the stage that is filled next
+                    ask(i + NST - 1);
+                    const int key0 = keys.x + (ub + i) * U + warp * KT, st = i % NST;
                     if (key0 >= keys.y) continue; // warp-uniform
-                    uint4 kr[NG][2][KL], vr[NG][4][VL];
-                    float ksc[NG], vsc[NG];
-                    bool have[NG];
-#pragma unroll
-                    for (int n = 0; n < NG; n++) {
-                        const int p = __shfl_sync(0xffffffffu, pg[n], i & 31), ib = __shfl_sync(0xffffffffu, inb[n], i & 31);
-                        have[n] = p >= 0;
-                        ksc[n] = vsc[n] = 1.f;
-                        if (have[n]) {
-                            const int64_t off = (int64_t)p * a.c.page_bytes + head_off + (int64_t)ib * (KQ_PAGE_BLOCK * HD * ES);
-                            const uint8_t *kp = a.c.k + off, *vp = a.c.v + off;
-                            if (F8) {
-                                const int64_t at = ((int64_t)p * a.c.n_kv + kh) * bpp + ib;
-                                ksc[n] = a.c.ks[at];
-                                vsc[n] = a.c.vs[at];
-                            }
-#pragma unroll
-                            for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                                for (int j = 0; j < KL; j++) kr[n][nt][j] = ld16(kp + (8 * nt + g) * (HD * ES) + 64 * j + 16 * t4);
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                const uint8_t *vrow = vp + (2 * t4 + (x & 1) + (x >> 1) * 8) * (HD * ES);
-                                if constexpr (HD * ES < 128) vr[n][x][0] = ld8(vrow + 8 * g);
-                                else {
-#pragma unroll
-                                    for (int j = 0; j < VL; j++) vr[n][x][j] = ld16(vrow + 128 * j + 16 * g);
-                                }
-                            }
-                        } else {
-#pragma unroll
-                            for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-                                for (int j = 0; j < KL; j++) kr[n][nt][j] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-                            for (int x = 0; x < 4; x++)
-#pragma unroll
-                                for (int j = 0; j < VL; j++) vr[n][x][j] = make_uint4(0, 0, 0, 0);
-                        }
-                    }
+                    const uint8_t *kst = ring + st * S::STEP, *vst = kst + KT * ROW;
+                    const int have = have_s[warp][st];
                     // ---- scores
                     float sc[NG][2][4];
 #pragma unroll
@@ -229,18 +247,16 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                             float(&c)[4] = sc[n][nt];
                             c[0] = c[1] = c[2] = c[3] = 0.f;
 #pragma unroll
-                            for (int ks = 0; ks < KS; ks++) {
-                                uint32_t b0, b1;
-                                if (F8) {
-                                    const uint32_t w = word(kr[n][nt][ks >> 2], ks & 3);
-                                    b0 = kq_e4m3x2_h2((uint16_t)w);
-                                    b1 = kq_e4m3x2_h2((uint16_t)(w >> 16));
-                                } else {
-                                    b0 = word(kr[n][nt][ks >> 1], 2 * (ks & 1));
-                                    b1 = word(kr[n][nt][ks >> 1], 2 * (ks & 1) + 1);
+                            for (int j = 0; j < KL; j++) {
+                                const uint4 kr = *reinterpret_cast<const uint4 *>(kst + place<ROW>(16 * n + 8 * nt + g, 4 * j + t4));
+#pragma unroll
+                                for (int x = 0; x < KS / KL; x++) {
+                                    const int ks = j * (KS / KL) + x;
+                                    const uint32_t b0 = F8 ? kq_e4m3x2_h2((uint16_t)word(kr, x)) : word(kr, 2 * x);
+                                    const uint32_t b1 = F8 ? kq_e4m3x2_h2((uint16_t)(word(kr, x) >> 16)) : word(kr, 2 * x + 1);
+                                    mma(c, qh[ks], b0, b1);
+                                    if (SPLIT) mma(c, ql[SPLIT ? ks : 0], b0, b1);
                                 }
-                                mma(c, qh[ks], b0, b1);
-                                if (SPLIT) mma(c, ql[SPLIT ? ks : 0], b0, b1);
                             }
                         }
                     float mx[HT];
@@ -249,10 +265,10 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
 #pragma unroll
                     for (int n = 0; n < NG; n++) {
                         const int kg = key0 + 16 * n;
-                        const bool all = have[n] && kg + 15 <= see_all && kg >= see_from;
+                        const bool all = (have >> n & 1) && kg + 15 <= see_all && kg >= see_from;
 #pragma unroll
                         for (int h = 0; h < HT; h++) {
-                            const float f = F8 ? crow[h] * ksc[n] : crow[h];
+                            const float f = F8 ? crow[h] * sc_s[warp][st][n] : crow[h];
 #pragma unroll
                             for (int nt = 0; nt < 2; nt++)
 #pragma unroll
@@ -261,21 +277,10 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                                     x *= f;
                                     if (!all) {
                                         const int key = kg + 8 * nt + 2 * t4 + j;
-                                        if (!have[n] || key > lim[h] || key >= keys.y || (a.window > 0 && key <= lim[h] - a.window)) x = -INFINITY;
+                                        if (!(have >> n & 1) || key > lim[h] || key >= keys.y || (a.window > 0 && key <= lim[h] - a.window)) x = -INFINITY;
                                     }
                                     mx[h] = fmaxf(mx[h], x);
                                 }
-                        }
-                        // a value that no row sees may hold anything: it must not meet a probability of 0
-                        if (have[n] && (kg + 16 > keys.y || kg < first_seen)) {
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                const int key = kg + 2 * t4 + (x & 1) + (x >> 1) * 8;
-                                if (key >= keys.y || key < first_seen) {
-#pragma unroll
-                                    for (int j = 0; j < VL; j++) vr[n][x][j] = make_uint4(0, 0, 0, 0);
-                                }
-                            }
                         }
                     }
                     // ---- softmax
@@ -286,8 +291,8 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                     for (int h = 0; h < HT; h++) {
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                        const float mn = fmaxf(m[h], mx[h]), sub = mn == -INFINITY ? 0.f : mn;
-                        alpha[h] = ex2(m[h] - sub); // nothing seen before: 2^-inf = 0
+                        const float mn = fmaxf(m[h], mx[h]), sub = mn == -INFINITY ? 0.f : mn - 14.f;
+                        alpha[h] = mn == -INFINITY ? 0.f : ex2(m[h] - mn); // nothing seen before: 2^-inf = 0
                         same = same && m[h] == mn;
                         m[h] = mn;
                         float sum = 0.f;
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                         for (int n = 0; n < NG; n++)
 #pragma unroll
                             for (int nt = 0; nt < 2; nt++) {
-                                const float p0 = ex2(sc[n][nt][2 * h] - sub), p1 = ex2(sc[n][nt][2 * h + 1] - sub);
+                                const float p0 = ex2(sc[n][nt][2 * h] - sub), p1 = ex2(sc[n][nt][2 * h + 1] - sub); // up to 2^14: small ones keep their bits in f16
                                 sum += p0 + p1;
                                 ph[n][h][nt] = h2(p0, p1);
                                 if (SPLIT) pl[SPLIT ? n : 0][h][nt] = h2_low(p0, p1, ph[n][h][nt]);
@@ -316,20 +321,39 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                         }
                     }
                     // ---- values
+                    uint4 vr[NG][4][VL];
 #pragma unroll
-                    for (int n = 0; n < NG; n++) {
-                        const __half2 vs2 = __float2half2_rn(vsc[n]);
+                    for (int n = 0; n < NG; n++)
 #pragma unroll
-                        for (int i = 0; i < MT; i++) {
+                        for (int x = 0; x < 4; x++) {
+                            const int r = 16 * n + 2 * t4 + (x & 1) + (x >> 1) * 8;
+                            if constexpr (ROW < 128) {
+                                const uint2 v = *reinterpret_cast<const uint2 *>(vst + place<ROW>(r, g >> 1) + 8 * (g & 1));
+                                vr[n][x][0] = make_uint4(v.x, v.y, 0, 0);
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < VL; j++) vr[n][x][j] = *reinterpret_cast<const uint4 *>(vst + place<ROW>(r, 8 * j + g));
+                            }
+                        }
+                    __half2 vs2[NG];
+#pragma unroll
+                    for (int n = 0; n < NG; n++) vs2[n] = __float2half2_rn(F8 && (have >> n & 1) ? sc_s[warp][st][2 + n] : 0.f);
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        float part[HT][4];
+#pragma unroll
+                        for (int h = 0; h < HT; h++) part[h][0] = part[h][1] = part[h][2] = part[h][3] = 0.f;
+#pragma unroll
+                        for (int n = 0; n < NG; n++) {
                             uint32_t va[4];
                             if (F8) { // two tiles per word of four dimensions
                                 const uint32_t pick = i & 1 ? 0x7362u : 0x5140u;
                                 const uint32_t x = __byte_perm(word(vr[n][0][0], i >> 1), word(vr[n][1][0], i >> 1), pick);
                                 const uint32_t y = __byte_perm(word(vr[n][2][0], i >> 1), word(vr[n][3][0], i >> 1), pick);
-                                va[0] = mul_h2(kq_e4m3x2_h2((uint16_t)x), vs2);
-                                va[1] = mul_h2(kq_e4m3x2_h2((uint16_t)(x >> 16)), vs2);
-                                va[2] = mul_h2(kq_e4m3x2_h2((uint16_t)y), vs2);
-                                va[3] = mul_h2(kq_e4m3x2_h2((uint16_t)(y >> 16)), vs2);
+                                va[0] = mul_h2(kq_e4m3x2_h2((uint16_t)x), vs2[n]);
+                                va[1] = mul_h2(kq_e4m3x2_h2((uint16_t)(x >> 16)), vs2[n]);
+                                va[2] = mul_h2(kq_e4m3x2_h2((uint16_t)y), vs2[n]);
+                                va[3] = mul_h2(kq_e4m3x2_h2((uint16_t)(y >> 16)), vs2[n]);
                             } else {
                                 const uint32_t w0 = word(vr[n][0][i >> 2], i & 3), w1 = word(vr[n][1][i >> 2], i & 3);
                                 const uint32_t w2 = word(vr[n][2][i >> 2], i & 3), w3 = word(vr[n][3][i >> 2], i & 3);
@@ -340,13 +364,23 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                             }
 #pragma unroll
                             for (int h = 0; h < HT; h++) {
-                                mma(o[h][i], va, ph[n][h][0], ph[n][h][1]);
-                                if (SPLIT) mma(o[h][i], va, pl[SPLIT ? n : 0][h][0], pl[SPLIT ? n : 0][h][1]);
+                                if (SPLIT) {
+                                    mma(part[h], va, pl[SPLIT ? n : 0][h][0], pl[SPLIT ? n : 0][h][1]);
+                                    mma(part[h], va, ph[n][h][0], ph[n][h][1]);
+                                } else mma(o[h][i], va, ph[n][h][0], ph[n][h][1]);
                             }
+                        }
+                        if (SPLIT) {
+#pragma unroll
+                            for (int h = 0; h < HT; h++)
+#pragma unroll
+                                for (int x = 0; x < 4; x++) o[h][i][x] += part[h][x];
                         }
                     }
                 }
+                copies_wait<0>();
                 // ---- the four warps' rows, joined in warp order
+                __syncwarp();
 #pragma unroll
                 for (int h = 0; h < HT; h++) {
                     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -358,8 +392,8 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
                         const int d = F8 ? (HD / 8) * g + 2 * i : 64 * (i >> 2) + 8 * g + 2 * (i & 3);
-                        *reinterpret_cast<float2 *>(&o_s[warp][8 * h + 2 * t4][d]) = make_float2(o[h][i][0], o[h][i][2]);
-                        *reinterpret_cast<float2 *>(&o_s[warp][8 * h + 2 * t4 + 1][d]) = make_float2(o[h][i][1], o[h][i][3]);
+                        *reinterpret_cast<float2 *>(&o_at(warp)[8 * h + 2 * t4][d]) = make_float2(o[h][i][0], o[h][i][2]);
+                        *reinterpret_cast<float2 *>(&o_at(warp)[8 * h + 2 * t4 + 1][d]) = make_float2(o[h][i][1], o[h][i][3]);
                     }
                 }
                 __syncthreads();
@@ -368,7 +402,8 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                 float *po = a.part + (int64_t)slot * R * (HD + 2), *pml = po + R * HD;
                 if (ub == 0 && !whole) {
                     const int per = (int)min((long long)0x7fffffff, run.u1 - run.u0); // a CTA whose item goes on has a full run
-                    meta = make_int4(1 + (int)(((long long)n_units - take + per - 1) / per), s, kh, tile);
+                    meta = make_int4(1 + (n_units - take + per - 1) / per, kh, tile, 0);
+                    meta2 = make_int4(sq.row0, sq.t, 0, 0);
                 }
                 for (int i = tid; i < R * (HD / 2); i += NT) {
                     const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
@@ -382,7 +417,7 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
 #pragma unroll
                     for (int w = 0; w < NW; w++) {
                         const float f = ex2(m_s[w][r] - sub);
-                        const float2 v = *reinterpret_cast<const float2 *>(&o_s[w][r][d]);
+                        const float2 v = *reinterpret_cast<const float2 *>(&o_at(w)[r][d]);
                         x += f * v.x;
                         y += f * v.y;
                         ll += f * l_s[w][r];
@@ -397,80 +432,122 @@ __global__ void __launch_bounds__(NT, HT == 1 ? 3 : 2) pages_decode_kernel(const
                 }
             }
     }
-    if (tid == 0) a.meta[blockIdx.x] = meta;
+    if (tid == 0) {
+        a.meta[2 * blockIdx.x] = meta;
+        a.meta[2 * blockIdx.x + 1] = meta2;
+    }
 }
 
-// CTA (b, row): one row of the item that begins in CTA b of the attention kernel and goes on in the next pieces - 1 of them.
-// 512 threads: groups of HD threads take every group-th piece.
-template <int HD> __global__ void __launch_bounds__(512) pages_combine_kernel(const __grid_constant__ KqAttnArgs a, int R) {
-    constexpr int NGRP = 512 / HD;
-    __shared__ float x_s[NGRP][HD], l_s[NGRP], m_s[16];
+// CTA b: the item of up to 16 rows that begins in CTA b of the attention kernel and goes on in the next pieces - 1 of them.  A row's pieces are
+// shared out over 512 / 32 / R warps, whose lanes are the dimensions; eight pieces' loads are in flight together.
+template <int HD, int R> __global__ void __launch_bounds__(512) pages_combine_kernel(const __grid_constant__ KqAttnArgs a) {
+    constexpr int W = 16 / R, N = HD / 64; // warps of a row, pairs of dimensions of a lane
+    __shared__ float2 o_s[16][HD / 2];
+    __shared__ float2 ml_s[16];
     KQ_PDL_ENTER();
-    const int4 meta = a.meta[blockIdx.x];
+    const int4 meta = a.meta[2 * blockIdx.x], seq = a.meta[2 * blockIdx.x + 1];
     if (meta.x == 0) return;
-    const KqSeq sq = kq_seq(a, meta.y);
-    const int r = blockIdx.y, rr = meta.w * R + r, tok = rr / a.G;
-    if (tok >= sq.t) return;
-    const int tid = threadIdx.x, d = tid % HD, grp = tid / HD;
-    const int64_t slot_floats = (int64_t)R * (HD + 2);
-    // piece 0 is slot 2 b + 1, piece i slot 2 (b + i)
-    auto piece = [&](int i) { return a.part + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * slot_floats; };
-    float mm = -INFINITY;
-    for (int i = tid; i < meta.x; i += 512) mm = fmaxf(mm, piece(i)[R * HD + 2 * r]);
-    mm = kq_warp_max(mm);
-    if ((tid & 31) == 0) m_s[tid >> 5] = mm;
-    __syncthreads();
-    mm = m_s[0];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = warp / W, part = warp % W;
+    float m = -INFINITY, l = 0.f;
+    float2 o[N];
 #pragma unroll
-    for (int w = 1; w < 16; w++) mm = fmaxf(mm, m_s[w]);
-    const float sub = mm == -INFINITY ? 0.f : mm;
-    float x = 0.f, l = 0.f;
-    for (int i0 = grp; i0 < meta.x; i0 += 8 * NGRP) {
-        float v[8];
-        float2 ml[8];
+    for (int u = 0; u < N; u++) o[u] = make_float2(0.f, 0.f);
+    for (int i0 = part; i0 < meta.x; i0 += 8 * W) {
+        float2 ml[8], v[8][N];
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const int i = i0 + j * NGRP;
-            v[j] = 0.f;
+            const int i = i0 + j * W;
             ml[j] = make_float2(-INFINITY, 0.f);
-            if (i < meta.x) {
-                const float *p = piece(i);
-                v[j] = p[r * HD + d];
+#pragma unroll
+            for (int u = 0; u < N; u++) v[j][u] = make_float2(0.f, 0.f);
+            if (i < meta.x) { // piece 0 is slot 2 b + 1, piece i slot 2 (b + i)
+                const float *p = a.part + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * (R * (HD + 2));
                 ml[j] = *reinterpret_cast<const float2 *>(p + R * HD + 2 * r);
+#pragma unroll
+                for (int u = 0; u < N; u++) v[j][u] = *reinterpret_cast<const float2 *>(p + r * HD + 2 * (lane + 32 * u));
             }
         }
+        float mn = m;
+#pragma unroll
+        for (int j = 0; j < 8; j++) mn = fmaxf(mn, ml[j].x);
+        const float sub = mn == -INFINITY ? 0.f : mn, f0 = ex2(m - sub);
+        l *= f0;
+#pragma unroll
+        for (int u = 0; u < N; u++) o[u].x *= f0, o[u].y *= f0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const float f = ex2(ml[j].x - sub);
-            x += f * v[j];
             l += f * ml[j].y;
+#pragma unroll
+            for (int u = 0; u < N; u++) o[u].x += f * v[j][u].x, o[u].y += f * v[j][u].y;
+        }
+        m = mn;
+    }
+    if (W > 1) { // the row's warps, in order
+#pragma unroll
+        for (int u = 0; u < N; u++) o_s[warp][lane + 32 * u] = o[u];
+        if (lane == 0) ml_s[warp] = make_float2(m, l);
+        __syncthreads();
+        if (part) return;
+        float mn = m;
+#pragma unroll
+        for (int w = 1; w < W; w++) mn = fmaxf(mn, ml_s[warp + w].x);
+        const float sub = mn == -INFINITY ? 0.f : mn, f0 = ex2(m - sub);
+        l *= f0;
+#pragma unroll
+        for (int u = 0; u < N; u++) o[u].x *= f0, o[u].y *= f0;
+#pragma unroll
+        for (int w = 1; w < W; w++) {
+            const float2 ml = ml_s[warp + w];
+            const float f = ex2(ml.x - sub);
+            l += f * ml.y;
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                const float2 v = o_s[warp + w][lane + 32 * u];
+                o[u].x += f * v.x, o[u].y += f * v.y;
+            }
         }
     }
-    x_s[grp][d] = x;
-    if (d == 0) l_s[grp] = l;
-    __syncthreads();
-    if (tid >= HD / 2) return;
-    float2 y = make_float2(0.f, 0.f);
-    float ll = 0.f;
+    const int rr = meta.z * R + r, tok = rr / a.G;
+    if (tok >= seq.y) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < NGRP; i++) {
-        y.x += x_s[i][2 * tid];
-        y.y += x_s[i][2 * tid + 1];
-        ll += l_s[i];
-    }
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    kq_st2_type(a.type, a.out, (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(meta.z * a.G + rr % a.G) * HD + 2 * tid, y.x * inv, y.y * inv);
+    for (int u = 0; u < N; u++)
+        kq_st2_type(a.type, a.out, (int64_t)(seq.x + tok) * a.out_stride + (int64_t)(meta.y * a.G + rr - tok * a.G) * HD + 2 * (lane + 32 * u), o[u].x * inv, o[u].y * inv);
 }
 
-template <int HD, bool F8, int HT, bool SPLIT> b200_status launch(const KqAttnArgs &a, int ctas, cudaStream_t st) {
-    kq_launch(pages_decode_kernel<HD, F8, HT, SPLIT>, ctas, NT, 0, st, a);
+b200_status combine(const KqAttnArgs &a, int hd, int R, int ctas, cudaStream_t st) {
+    kq_launch(hd == 128 ? (R == 8 ? pages_combine_kernel<128, 8> : pages_combine_kernel<128, 16>) : (R == 8 ? pages_combine_kernel<64, 8> : pages_combine_kernel<64, 16>), ctas, 512,
+              0, st, a);
     KQ_COUNT_LAUNCH();
     KQ_LAUNCH_CHECK();
     return B200_OK;
 }
-template <int HD, bool F8> b200_status launch(const KqAttnArgs &a, int ht, bool split, int ctas, cudaStream_t st) {
-    if (ht == 1) return split ? launch<HD, F8, 1, true>(a, ctas, st) : launch<HD, F8, 1, false>(a, ctas, st);
-    return split ? launch<HD, F8, 2, true>(a, ctas, st) : launch<HD, F8, 2, false>(a, ctas, st);
+
+template <int HD, bool F8, int HT, typename T> b200_status launch(const KqAttnArgs &a, cudaStream_t st, int *ctas) {
+    using S = Shape<HD, F8, HT>;
+    static bool attr[64];
+    int dev = 0;
+    KQ_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64 || !attr[dev]) {
+        KQ_CUDA(cudaFuncSetAttribute(pages_decode_kernel<HD, F8, HT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+        if (dev >= 0 && dev < 64) attr[dev] = true;
+    }
+    *ctas = kq_sm_count() * S::CTAS;
+    kq_launch(pages_decode_kernel<HD, F8, HT, T>, *ctas, NT, S::SMEM, st, a);
+    KQ_COUNT_LAUNCH();
+    KQ_LAUNCH_CHECK();
+    return B200_OK;
+}
+template <int HD, bool F8, int HT> b200_status launch(const KqAttnArgs &a, cudaStream_t st, int *ctas) {
+    if (a.type == B200_TYPE_F32) return launch<HD, F8, HT, float>(a, st, ctas);
+    return a.type == B200_TYPE_F16 ? launch<HD, F8, HT, __half>(a, st, ctas) : launch<HD, F8, HT, __nv_bfloat16>(a, st, ctas);
+}
+template <int HD> b200_status launch(const KqAttnArgs &a, bool f8, int ht, cudaStream_t st) {
+    int ctas = 0;
+    if (f8) KQ_TRY(ht == 1 ? (launch<HD, true, 1>(a, st, &ctas)) : (launch<HD, true, 2>(a, st, &ctas)));
+    else KQ_TRY(ht == 1 ? (launch<HD, false, 1>(a, st, &ctas)) : (launch<HD, false, 2>(a, st, &ctas)));
+    return combine(a, HD, 8 * ht, ctas, st);
 }
 
 // Sequences of up to FEW rows of a KV head go to the kernel above, longer ones to the one for prompts, where the caller says there are any
@@ -481,27 +558,16 @@ constexpr size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 } // namespace
 
-b200_status kq_pages_combine(const KqAttnArgs &a, int hd, int R, int ctas, cudaStream_t st) {
-    const dim3 grid((unsigned)ctas, (unsigned)R);
-    kq_launch(hd == 128 ? pages_combine_kernel<128> : pages_combine_kernel<64>, grid, 512, 0, st, a, R);
-    KQ_COUNT_LAUNCH();
-    KQ_LAUNCH_CHECK();
-    return B200_OK;
-}
-
 size_t kq_pages_decode_scratch(int hd) {
     const size_t ctas = (size_t)kq_sm_count() * MAX_CTAS_PER_SM;
-    return up256(ctas * sizeof(int4)) + ctas * 2 * 16 * (hd + 2) * sizeof(float);
+    return up256(ctas * 2 * sizeof(int4)) + ctas * 2 * 16 * (hd + 2) * sizeof(float);
 }
 
 b200_status kq_pages_decode(KqAttnArgs a, bool f8, int hd, int64_t most, uint8_t *scratch, cudaStream_t st) {
-    const bool split = a.type == B200_TYPE_F32;
-    const int ht = most <= 8 ? 1 : 2, ctas = kq_sm_count() * (ht == 1 ? 3 : 2);
+    const int ht = most <= 8 ? 1 : 2;
     a.meta = (int4 *)scratch;
-    a.part = (float *)(scratch + up256((size_t)kq_sm_count() * MAX_CTAS_PER_SM * sizeof(int4)));
-    if (hd == 128) KQ_TRY(f8 ? (launch<128, true>(a, ht, split, ctas, st)) : (launch<128, false>(a, ht, split, ctas, st)));
-    else KQ_TRY(f8 ? (launch<64, true>(a, ht, split, ctas, st)) : (launch<64, false>(a, ht, split, ctas, st)));
-    return kq_pages_combine(a, hd, 8 * ht, ctas, st);
+    a.part = (float *)(scratch + up256((size_t)kq_sm_count() * MAX_CTAS_PER_SM * 2 * sizeof(int4)));
+    return hd == 128 ? launch<128>(a, f8, ht, st) : launch<64>(a, f8, ht, st);
 }
 
 extern "C" {

@@ -3,8 +3,7 @@
 // A CTA works on two tiles of 128 rows (row i of a sequence and KV head: token i / G, head i % G) that share every tile of 128 keys: while
 // the tensor cores multiply for one, the softmax warps of the other work.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with S (columns
 // 0 and 128) and O (256 and 384) in TMEM; a softmax thread owns a row: it writes its probabilities over scores that it has read, as f16, which
-// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 8 in base 2 (a
-// probability then is at most 2^8, far from f16's end).  f32 queries go in as two f16 parts, and so do their probabilities; f16 queries, which the rotation makes longer than f16, go in as two.  As in the kernel for few rows a query row is
+// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 8 in base 2.  f32 queries go in as two f16 parts, and so do their probabilities; f16 queries, which the rotation makes longer than f16, go in as two.  As in the kernel for few rows a query row is
 // divided by the power of two of its largest element.
 //
 // K and V tiles go through a ring in the order K0 V0 K1 V1 ...; f16 pages arrive by tiled TMA, 64 dimensions x 16 .. 128 positions of a page
@@ -20,6 +19,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 b200_status kq_tmap_encode(void *map128, int elem_bytes, int rank, const void *base, const uint64_t *dims, const uint64_t *strides_bytes, const uint32_t *box, int swizzle128);
 
 namespace {
@@ -27,6 +28,11 @@ namespace {
 constexpr int R = 256, BK = 128, NSOFT = 256;
 constexpr uint64_t LIMIT = 5 * KQ_WAIT_LIMIT_NS;
 constexpr uint32_t COL_S = 0, COL_O = 256;
+// f32: the tensor cores cut their sums off instead of rounding them, each step of 16 keys and part by half a last bit on average, which made rows
+// of 1800 keys to a piece 4e-6 too small.  So the row's sum of probabilities is cut off in the same steps (what is lost cancels where it is
+// divided by), and every FLUSH units O and the sum are put aside and added up in 32 bits.
+constexpr int FLUSH = 16;
+constexpr float CUT_HALF_BIT = 4.3e-8f; // half a last bit relative to the value, over mantissas of 1 to 2 as they come: 2^-24 / (2 ln 2)
 
 __device__ int g_pages_error;
 
@@ -106,6 +112,7 @@ constexpr int MAX_SLOTS = 6;
 struct Shared {
     uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_done, q_ready;
     float crow[R];
+    double turns[64]; // a lane's own entry is no broadcast: not from the constant bank
     uint32_t tmem;
     int abort;
 };
@@ -122,9 +129,8 @@ struct Walk {
         s = run.s;
         if (u >= u1) return;
         sq = kq_seq(a, s);
-        const long long per_head = kq_head_units<R, BK>(a, sq);
-        kh = (int)(run.off / per_head);
-        uo = run.off % per_head;
+        kh = (int)kq_div(run.off, run.per_head);
+        uo = run.off - kh * run.per_head;
         tiles = kq_tiles<R>(a, sq.t);
         for (tile = 0;; tile++) {
             n_units = kq_units<BK>(kq_tile_keys<R>(a, sq, tile));
@@ -169,9 +175,11 @@ __device__ __forceinline__ uint4 decode8(uint32_t lo, uint32_t hi, __half2 s) {
     return make_uint4(two(lo), two(lo >> 16), two(hi), two(hi >> 16));
 }
 
-template <int HD, bool F8, int QS, int PS>
+// T: the activations' type; f32 and f16 queries in two f16 parts, probabilities of f32 results in two
+template <int HD, bool F8, typename T>
 __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     pages_prompt_kernel(const __grid_constant__ KqAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box_rows) {
+    constexpr int QS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PS = std::is_same<T, float>::value ? 2 : 1;
     using L = Layout<HD, F8, QS>;
     constexpr int NS = L::NS, NR = L::NR > 0 ? L::NR : 1, NT = F8 ? 512 : 384;
     extern __shared__ __align__(1024) uint8_t sm_raw[];
@@ -182,6 +190,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    if (tid < HD / 2) sh.turns[tid] = a.turns.f[tid];
     if (tid == 0) {
         auto init = [](uint64_t &b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&b)), "r"(n)); };
         for (int i = 0; i < MAX_SLOTS; i++) {
@@ -207,6 +216,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     const uint32_t tmem = sh.tmem;
     volatile int *abort = &sh.abort;
     auto wait = [&](uint64_t &bar, uint32_t parity, int code) {
+        for (int i = 0; i < 32; i++) // the clock is read only when it takes longer
+            if (kq_mbar_try(smem_u32(&bar), parity)) return;
         if (!*abort && !kq_mbar_wait(smem_u32(&bar), parity, LIMIT)) {
             *abort = 1;
             atomicExch(&g_pages_error, code);
@@ -217,7 +228,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     Walk w;
     w.start(a, run);
     const int bpp = a.c.page / KQ_PAGE_BLOCK;
-    int4 meta = make_int4(0, 0, 0, 0);
+    int4 meta = make_int4(0, 0, 0, 0), meta2 = meta;
 
     if (warp == 8) {
         // ---------------------------------------------------------------- products
@@ -257,7 +268,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     wait(sh.p_ready[0], units & 1, 3);
                     wait(sh.full[v % NS], (v / NS) & 1, 4);
                     after_sync();
-                    values(0, v, i == 0);
+                    values(0, v, PS == 2 ? i % FLUSH == 0 : i == 0);
                     if (more) {
                         wait(sh.full[k % NS], (k / NS) & 1, 5);
                         after_sync();
@@ -266,7 +277,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     }
                     wait(sh.p_ready[1], units & 1, 6);
                     after_sync();
-                    values(1, v, i == 0);
+                    values(1, v, PS == 2 ? i % FLUSH == 0 : i == 0);
                     commit(smem_u32(&sh.empty[v % NS]));
                     if (more) {
                         scores(1, k);
@@ -394,36 +405,44 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
             for (int u = 0; u < P; u++) cs[u] = make_float2(1.f, 0.f);
             // the lane's pairs are P lane + u: dimensions (pair, pair + HD / 2) or (2 pair, 2 pair + 1)
+            int tok = (row0 + (warp & 3) * 32) / a.G, h = row0 + (warp & 3) * 32 - tok * a.G; // of the next row
+#pragma unroll 1
             for (int rb = 0; rb < 32; rb += 4) {
                 float x[4][P][2];
+                int toks[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const int rr = row0 + (warp & 3) * 32 + rb + k, tok = rr / a.G;
+                    toks[k] = tok;
 #pragma unroll
                     for (int u = 0; u < P; u++) x[k][u][0] = x[k][u][1] = 0.f;
-                    if (tok >= w.sq.t) continue;
-                    const int64_t at = (int64_t)(w.sq.row0 + tok) * a.q_stride + (int64_t)(w.kh * a.G + rr % a.G) * HD;
-                    if (split && P == 2) {
-                        const float2 v0 = kq_ld2_type(a.type, a.q, at + 2 * lane), v1 = kq_ld2_type(a.type, a.q, at + HD / 2 + 2 * lane);
-                        x[k][0][0] = v0.x, x[k][P - 1][0] = v0.y, x[k][0][1] = v1.x, x[k][P - 1][1] = v1.y;
-                    } else if (split) {
-                        x[k][0][0] = kq_ld1_type(a.type, a.q, at + lane);
-                        x[k][0][1] = kq_ld1_type(a.type, a.q, at + HD / 2 + lane);
-                    } else {
+                    if (tok < w.sq.t) {
+                        const T *q = (const T *)a.q + (int64_t)(w.sq.row0 + tok) * a.q_stride + (int64_t)(w.kh * a.G + h) * HD;
+                        if (split && P == 2) {
+                            const float2 v0 = kq_ld2(q + 2 * lane), v1 = kq_ld2(q + HD / 2 + 2 * lane);
+                            x[k][0][0] = v0.x, x[k][P - 1][0] = v0.y, x[k][0][1] = v1.x, x[k][P - 1][1] = v1.y;
+                        } else if (split) {
+                            x[k][0][0] = kq_ld1(q + lane);
+                            x[k][0][1] = kq_ld1(q + HD / 2 + lane);
+                        } else {
 #pragma unroll
-                        for (int u = 0; u < P; u++) {
-                            const float2 v = kq_ld2_type(a.type, a.q, at + 2 * (P * lane + u));
-                            x[k][u][0] = v.x, x[k][u][1] = v.y;
+                            for (int u = 0; u < P; u++) {
+                                const float2 v = kq_ld2(q + 2 * (P * lane + u));
+                                x[k][u][0] = v.x, x[k][u][1] = v.y;
+                            }
                         }
+                    }
+                    if (++h == a.G) {
+                        h = 0;
+                        tok++;
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const int r = (warp & 3) * 32 + rb + k, rr = row0 + r, tok = rr / a.G;
-                    if (a.turns.on && tok != tok_cs && tok < w.sq.t) {
-                        tok_cs = tok;
+                    const int r = (warp & 3) * 32 + rb + k;
+                    if (a.turns.on && toks[k] != tok_cs && toks[k] < w.sq.t) {
+                        tok_cs = toks[k];
 #pragma unroll
-                        for (int u = 0; u < P; u++) cs[u] = kq_turn(a.turns.f[P * lane + u], w.sq.pos(tok));
+                        for (int u = 0; u < P; u++) cs[u] = kq_turn_call(sh.turns[P * lane + u], w.sq.pos(tok_cs));
                     }
                     float amax = 0.f;
 #pragma unroll
@@ -471,7 +490,25 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             };
             uint32_t there = 0;
             int ahead = look_up(0);
-            float m = -INFINITY, l = 0.f;
+            const int slot = 2 * blockIdx.x + (w.ub == 0 ? 1 : 0); // of a piece that is not the whole item, and of sums on their way
+            float *part = a.part + (int64_t)slot * R * (HD + 2) + (int64_t)(128 * half + row) * HD;
+            float m = -INFINITY, l = 0.f, l_sum = 0.f, m_sum = -INFINITY; // l_sum: of what was put aside; m_sum: the maximum that it goes by
+            // the row's O so far: what the tensor cores have summed and what was put aside before; as 32 columns a time
+            auto total = [&](int k, uint32_t *o) {
+                tmem_ld32(to + 32 * k, o);
+                tmem_ld_wait();
+                if (PS == 2 && m_sum != -INFINITY) {
+                    const float f = ex2(m_sum - m);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(part + 32 * k + j);
+                        o[j] = __float_as_uint(fmaf(v.x, f, __uint_as_float(o[j])));
+                        o[j + 1] = __float_as_uint(fmaf(v.y, f, __uint_as_float(o[j + 1])));
+                        o[j + 2] = __float_as_uint(fmaf(v.z, f, __uint_as_float(o[j + 2])));
+                        o[j + 3] = __float_as_uint(fmaf(v.w, f, __uint_as_float(o[j + 3])));
+                    }
+                }
+            };
             for (int i = 0; i < w.take; i++, units++) {
                 if ((i & 3) == 0) {
                     there = __ballot_sync(0xffffffffu, ahead >= 0);
@@ -480,7 +517,20 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 const uint32_t blocks = (there >> (8 * (i & 3))) & 0xff;
                 const int key0 = w.keys.x + (w.ub + i) * BK;
                 wait(sh.s_ready[half], units & 1, 10);
-                after_sync();
+                after_sync(); // S was issued behind the products before: O is at rest
+                if (PS == 2 && i > 0 && i % FLUSH == 0) {
+#pragma unroll
+                    for (int k = 0; k < HD / 32; k++) {
+                        uint32_t o[32];
+                        total(k, o);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<uint4 *>(part + 32 * k + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    }
+                    l_sum = l + (m_sum != -INFINITY ? l_sum * ex2(m_sum - m) : 0.f);
+                    l = 0.f;
+                    m_sum = m;
+                }
                 // the scores are read twice, 32 at a time (the maximum, then the probabilities): a row of 128 would not fit next to the rest
                 const bool masked = blocks != 0xff || key0 + BK - 1 > lim_lo || (a.window > 0 && key0 <= lim_hi - a.window);
                 const int last = lim - key0, first = a.window > 0 ? last - a.window + 1 : -0x7fffffff;
@@ -505,7 +555,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 if (__any_sync(0xffffffffu, grown)) {
                     const float mn = grown ? fmaxf(m, top) : m, alpha = mn == m ? 1.f : ex2(m - mn);
                     m = mn;
-                    if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) { // S of this tile was issued behind the product before: O is at rest
+                    if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                         l *= alpha;
 #pragma unroll
                         for (int k = 0; k < HD / 32; k++) {
@@ -518,7 +568,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         }
                     }
                 }
-                const float sub = m == -INFINITY ? 0.f : m;
+                const float sub = m == -INFINITY ? 0.f : m - 6.f; // probabilities up to 2^14: small ones keep their bits in f16
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
                 uint32_t lo_even[PS == 2 ? 16 : 1];
                 // a chunk's probabilities go over scores that have been read: those of keys 0 .. 63 to columns 0 .. 31 (second parts 32 .. 63) ...
@@ -532,9 +582,13 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         const float p0 = ex2(fmaf(__uint_as_float(x[2 * j]), crow, -sub)), p1 = ex2(fmaf(__uint_as_float(x[2 * j + 1]), crow, -sub));
-                        sum[j & 3] += p0 + p1;
+                        sum[PS == 2 ? j >> 3 : j & 3] += p0 + p1;
                         hi[j] = h2(p0, p1);
                         if (PS == 2) lo[PS == 2 ? j : 0] = h2_low(p0, p1, hi[j]);
+                    }
+                    if (PS == 2) {
+                        l = __fadd_rz(__fadd_rz(l, sum[0]), sum[1]);
+                        sum[0] = sum[1] = 0.f;
                     }
                     if (PS == 2 && (c & 1) == 0) {
 #pragma unroll
@@ -548,7 +602,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         }
                     }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (PS == 2) l = fmaf(l, -8.f * CUT_HALF_BIT, l); // the second parts' eight steps
+                else l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (!F8 && half == 0 && (key0 + BK > w.keys.y || key0 < seen)) {
                     // a value that no row sees may hold anything: it must not meet a probability of 0
                     const uint32_t v = 2 * units + 1;
@@ -567,47 +622,65 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             // ---- results
             wait(sh.o_done, pieces & 1, 12);
             after_sync();
+            if (PS == 2 && m_sum != -INFINITY) l = fmaf(l_sum, ex2(m_sum - m), l);
             const bool whole = w.ub == 0 && w.take == w.n_units, ok = (row0 + row) / a.G < w.sq.t && !*abort;
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-            const int64_t at = whole ? (int64_t)(w.sq.row0 + my_tok) * a.out_stride + (int64_t)(w.kh * a.G + (row0 + row) % a.G) * HD
-                                     : (int64_t)(2 * blockIdx.x + (w.ub == 0 ? 1 : 0)) * R * (HD + 2) + (int64_t)(128 * half + row) * HD;
-#pragma unroll
+            // 32 columns a time through the warp's part of the queries' room, so that a store writes whole lines of 4 rows
+            uint8_t *turn = sm + half * L::TILE + (warp & 3) * 4096;
+            const int cr = lane >> 3, cc = lane & 7; // row of four and 16-byte chunk of a store
+            const int wr0 = row0 + (warp & 3) * 32, wtok0 = wr0 / a.G, wh0 = wr0 - wtok0 * a.G;
+#pragma unroll 1
             for (int k = 0; k < HD / 32; k++) {
                 uint32_t o[32];
-                tmem_ld32(to + 32 * k, o);
-                tmem_ld_wait();
-                if (!ok) continue;
+                total(k, o);
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    float v[8];
+                for (int j = 0; j < 8; j++) {
+                    float4 v;
+                    v.x = __uint_as_float(o[4 * j]) * inv, v.y = __uint_as_float(o[4 * j + 1]) * inv, v.z = __uint_as_float(o[4 * j + 2]) * inv, v.w = __uint_as_float(o[4 * j + 3]) * inv;
+                    if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    *reinterpret_cast<float4 *>(turn + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+                }
+                __syncwarp();
 #pragma unroll
-                    for (int x = 0; x < 8; x++) v[x] = l == 0.f ? 0.f : __uint_as_float(o[j + x]) * inv; // nothing seen: O is 0 by zeros
-                    if (!whole || a.type == B200_TYPE_F32) {
-                        float *p = (whole ? (float *)a.out : a.part) + at + 32 * k + j;
-                        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-                        *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                    } else {
-                        uint4 u;
-                        if (a.type == B200_TYPE_F16) u = make_uint4(h2(v[0], v[1]), h2(v[2], v[3]), h2(v[4], v[5]), h2(v[6], v[7]));
+                for (int j = 0; j < 8; j++) {
+                    const int r = 4 * j + cr; // of the warp's 32 rows
+                    const float4 v = *reinterpret_cast<const float4 *>(turn + r * 128 + ((cc ^ (r & 7)) << 4));
+                    int tok = wtok0, h = wh0 + r;
+                    if (h >= a.G) {
+                        tok += h / a.G;
+                        h %= a.G;
+                    }
+                    if (tok >= w.sq.t || *abort) continue;
+                    if (!whole) *reinterpret_cast<float4 *>(a.part + (int64_t)slot * R * (HD + 2) + (int64_t)(128 * half + (warp & 3) * 32 + r) * HD + 32 * k + 4 * cc) = v;
+                    else {
+                        T *out = (T *)a.out + (int64_t)(w.sq.row0 + tok) * a.out_stride + (int64_t)(w.kh * a.G + h) * HD + 32 * k + 4 * cc;
+                        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out) = v;
+                        else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<uint2 *>(out) = make_uint2(h2(v.x, v.y), h2(v.z, v.w));
                         else {
-                            const __nv_bfloat162 b[4] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3]), __floats2bfloat162_rn(v[4], v[5]),
-                                                         __floats2bfloat162_rn(v[6], v[7])};
-                            u = *reinterpret_cast<const uint4 *>(b);
+                            const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
+                            *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(b);
                         }
-                        *reinterpret_cast<uint4 *>((uint16_t *)a.out + at + 32 * k + j) = u;
                     }
                 }
             }
+            __syncwarp(); // the next item's queries go where the rows went through
             if (!whole && ok) {
-                float *ml = a.part + (int64_t)(2 * blockIdx.x + (w.ub == 0 ? 1 : 0)) * R * (HD + 2) + (int64_t)R * HD + 2 * (128 * half + row);
+                float *ml = a.part + (int64_t)slot * R * (HD + 2) + (int64_t)R * HD + 2 * (128 * half + row);
                 *reinterpret_cast<float2 *>(ml) = make_float2(m, l);
             }
-            if (tid == 0 && w.ub == 0 && !whole) meta = make_int4(1 + (int)((w.n_units - w.take + (run.u1 - run.u0) - 1) / (run.u1 - run.u0)), w.s, w.kh, w.tile);
+            if (w.ub == 0 && !whole) {
+                meta = make_int4(1 + (int)kq_div(w.n_units - w.take + (run.u1 - run.u0) - 1, run.u1 - run.u0), w.kh, w.tile, 0);
+                meta2 = make_int4(w.sq.row0, w.sq.t, 0, 0);
+            }
             before_sync();
             pieces++;
             w.done();
         }
-        if (tid == 0) a.meta[blockIdx.x] = meta;
+        if (tid == 0) {
+            a.meta[2 * blockIdx.x] = meta;
+            a.meta[2 * blockIdx.x + 1] = meta2;
+        }
     }
     before_sync();
     __syncthreads();
@@ -617,15 +690,14 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 // joins the pieces of a split item: a warp per row, lanes the dimensions; grid (CTAs of the attention kernel, R / 16)
 template <int HD> __global__ void __launch_bounds__(256) pages_join_kernel(const __grid_constant__ KqAttnArgs a) {
     KQ_PDL_ENTER();
-    const int4 meta = a.meta[blockIdx.x];
+    const int4 meta = a.meta[2 * blockIdx.x], seq = a.meta[2 * blockIdx.x + 1];
     if (meta.x == 0) return;
-    const KqSeq sq = kq_seq(a, meta.y);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     constexpr int N = HD / 64;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const int r = blockIdx.y * 16 + 2 * warp + k, rr = meta.w * R + r, tok = rr / a.G;
-        if (tok >= sq.t) continue;
+        const int r = blockIdx.y * 16 + 2 * warp + k, rr = meta.z * R + r, tok = rr / a.G;
+        if (tok >= seq.y) continue;
         float m = -INFINITY, l = 0.f;
         float2 o[N];
 #pragma unroll
@@ -662,30 +734,30 @@ template <int HD> __global__ void __launch_bounds__(256) pages_join_kernel(const
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int u = 0; u < N; u++)
-            kq_st2_type(a.type, a.out, (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(meta.z * a.G + rr % a.G) * HD + 2 * (lane + 32 * u), o[u].x * inv, o[u].y * inv);
+            kq_st2_type(a.type, a.out, (int64_t)(seq.x + tok) * a.out_stride + (int64_t)(meta.y * a.G + rr - tok * a.G) * HD + 2 * (lane + 32 * u), o[u].x * inv, o[u].y * inv);
     }
 }
 
-template <int HD, bool F8, int QS, int PS> b200_status launch(const KqAttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int box_rows, int ctas, cudaStream_t st) {
+template <int HD, bool F8, typename T> b200_status launch(const KqAttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int box_rows, int ctas, cudaStream_t st) {
+    constexpr int smem = Layout<HD, F8, std::is_same<T, __nv_bfloat16>::value ? 1 : 2>::TOTAL;
     static bool attr[64];
     int dev = 0;
     KQ_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !attr[dev]) {
-        KQ_CUDA(cudaFuncSetAttribute(pages_prompt_kernel<HD, F8, QS, PS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<HD, F8, QS>::TOTAL));
+        KQ_CUDA(cudaFuncSetAttribute(pages_prompt_kernel<HD, F8, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         if (dev >= 0 && dev < 64) attr[dev] = true;
     }
-    kq_launch(pages_prompt_kernel<HD, F8, QS, PS>, ctas, F8 ? 512 : 384, Layout<HD, F8, QS>::TOTAL, st, a, k, v, box_rows);
+    kq_launch(pages_prompt_kernel<HD, F8, T>, ctas, F8 ? 512 : 384, smem, st, a, k, v, box_rows);
     KQ_COUNT_LAUNCH();
     KQ_LAUNCH_CHECK();
     return B200_OK;
 }
 template <int HD, bool F8> b200_status launch(const KqAttnArgs &a, const CUtensorMap &k, const CUtensorMap &v, int box_rows, int ctas, cudaStream_t st) {
-    if (a.type == B200_TYPE_F32) return launch<HD, F8, 2, 2>(a, k, v, box_rows, ctas, st);
-    if (a.type == B200_TYPE_F16 && a.turns.on) return launch<HD, F8, 2, 1>(a, k, v, box_rows, ctas, st);
-    return launch<HD, F8, 1, 1>(a, k, v, box_rows, ctas, st);
+    if (a.type == B200_TYPE_F32) return launch<HD, F8, float>(a, k, v, box_rows, ctas, st);
+    return a.type == B200_TYPE_F16 ? launch<HD, F8, __half>(a, k, v, box_rows, ctas, st) : launch<HD, F8, __nv_bfloat16>(a, k, v, box_rows, ctas, st);
 }
 
-constexpr size_t META_BYTES = 4096;
+constexpr size_t META_BYTES = 8192;
 
 } // namespace
 
@@ -700,7 +772,7 @@ size_t kq_pages_prompt_scratch(int hd) { return META_BYTES + (size_t)kq_sm_count
 
 b200_status kq_pages_prompt(KqAttnArgs a, bool f8, int hd, uint8_t *scratch, cudaStream_t st) {
     const int ctas = kq_sm_count();
-    KQ_REQUIRE((size_t)ctas * sizeof(int4) <= META_BYTES, "attention_pages: %d multiprocessors", ctas);
+    KQ_REQUIRE((size_t)ctas * 2 * sizeof(int4) <= META_BYTES, "attention_pages: %d multiprocessors", ctas);
     a.meta = (int4 *)scratch;
     a.part = (float *)(scratch + META_BYTES);
     int box_rows = 128; // the largest power of two that divides the page

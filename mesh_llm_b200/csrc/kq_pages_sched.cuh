@@ -20,7 +20,7 @@ struct KqAttnArgs {
     float scale_log2;
     KqTurns turns;
     float *part; // [2 CTAs][R][HD + 2]: unnormalised rows, then (maximum, sum) of each
-    int4 *meta;  // [CTAs]: pieces (0: none), sequence, KV head, tile
+    int4 *meta;  // [CTAs][2]: pieces (0: none), KV head, tile, -; first row and number of rows of the sequence, -, -
 };
 
 #ifdef __CUDACC__
@@ -44,25 +44,50 @@ template <int R> __device__ __forceinline__ int2 kq_tile_keys(const KqAttnArgs &
     return make_int2(min(lo, hi & ~(A - 1)), hi);
 }
 template <int U> __device__ __forceinline__ int kq_units(int2 keys) { return max(1, (keys.y - keys.x + U - 1) / U); }
+// units of one KV head of a sequence; the tiles' last tokens are counted on, not divided out
 template <int R, int U> __device__ __forceinline__ long long kq_head_units(const KqAttnArgs &a, const KqSeq &q) {
-    long long n = 0;
     const int tiles = kq_tiles<R>(a, q.t);
-    for (int i = 0; i < tiles; i++) n += kq_units<U>(kq_tile_keys<R>(a, q, i));
+    if (tiles <= 1 || a.window > 0) {
+        long long n = 0;
+        for (int i = 0; i < tiles; i++) n += kq_units<U>(kq_tile_keys<R>(a, q, i));
+        return n;
+    }
+    if (q.p0 < 0) return tiles;
+    long long n = 0;
+    const int64_t cap = (int64_t)a.c.table_len * a.c.page;
+    const int dq = R / a.G, dr = R % a.G;
+    int last = (R - 1) / a.G, rem = (R - 1) % a.G;
+#pragma unroll 4
+    for (int i = 0; i < tiles; i++) {
+        n += (uint32_t)(max(min((int64_t)q.p0 + min(last, q.t - 1) + 1, cap), (int64_t)1) + U - 1) / (uint32_t)U;
+        last += dq;
+        rem += dr;
+        if (rem >= a.G) {
+            rem -= a.G;
+            last++;
+        }
+    }
     return n;
 }
 
+// counts fit 32 bits but for absurd batches
+__device__ __forceinline__ long long kq_div(long long a, long long b) { return ((a | b) >> 31) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b; }
+
 // this CTA's run of units: [u0, u1), beginning `off` units into sequence s
 struct KqRun {
-    long long u0, u1, off;
+    long long u0, u1, off, per_head; // per_head: units of a KV head of s
     int s;
 };
 template <int R, int U, int NT> __device__ KqRun kq_find_run(const KqAttnArgs &a) {
-    __shared__ long long warp_sum[NT / 32], s_off;
+    __shared__ long long warp_sum[NT / 32], s_off, s_head;
     __shared__ int s_seq;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = (a.b.n_seq + NT - 1) / NT, i0 = min(a.b.n_seq, tid * each), i1 = min(a.b.n_seq, i0 + each);
-    long long sum = 0;
-    for (int i = i0; i < i1; i++) sum += kq_head_units<R, U>(a, kq_seq(a, i)) * a.c.n_kv;
+    long long sum = 0, head = 0;
+    for (int i = i0; i < i1; i++) {
+        head = kq_head_units<R, U>(a, kq_seq(a, i));
+        sum += head * a.c.n_kv;
+    }
     long long inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -78,29 +103,30 @@ template <int R, int U, int NT> __device__ KqRun kq_find_run(const KqAttnArgs &a
         if (w < warp) before += warp_sum[w];
         total += warp_sum[w];
     }
-    const long long per = max(1ll, (total + gridDim.x - 1) / (long long)gridDim.x), u0 = per * blockIdx.x;
+    const long long per = max(1ll, kq_div(total + gridDim.x - 1, gridDim.x)), u0 = per * blockIdx.x;
     if (u0 >= before && u0 < before + sum) {
         long long off = u0 - before;
         for (int i = i0; i < i1; i++) {
-            const long long n = kq_head_units<R, U>(a, kq_seq(a, i)) * a.c.n_kv;
+            const long long h = i1 - i0 == 1 ? head : kq_head_units<R, U>(a, kq_seq(a, i)), n = h * a.c.n_kv;
             if (off < n) {
                 s_seq = i;
                 s_off = off;
+                s_head = h;
                 break;
             }
             off -= n;
         }
     }
     __syncthreads();
-    KqRun r{u0, min(total, u0 + per), 0, s_seq};
-    if (r.s < a.b.n_seq) r.off = s_off;
-    else r.u1 = r.u0;
+    KqRun r{u0, min(total, u0 + per), 0, 1, s_seq};
+    if (r.s < a.b.n_seq) {
+        r.off = s_off;
+        r.per_head = s_head;
+    } else r.u1 = r.u0;
     return r;
 }
 #endif
 
-// joins the pieces of split items; grid (CTAs of the attention kernel, rows of a tile)
-b200_status kq_pages_combine(const KqAttnArgs &a, int hd, int R, int ctas, cudaStream_t st);
 // sequences of few rows (any number is right), and its workspace
 size_t kq_pages_decode_scratch(int hd);
 b200_status kq_pages_decode(KqAttnArgs a, bool f8, int hd, int64_t most, uint8_t *scratch, cudaStream_t st);
