@@ -26,8 +26,8 @@ struct KqBatch {
     const int32_t *row_start, *pos0;
     int32_t rows, n_seq;
 };
-struct KqTurns { // turns per position of each rotated pair, 0: keys and queries are used as they come
-    double f[64];
+struct KqTurns { // turns per position of each rotated pair in units of 2^-64; on = 0: keys and queries are used as they come
+    uint64_t f[64];
     int32_t on, neox;
 };
 
@@ -37,18 +37,15 @@ b200_status kq_rows_check(const char *who, const char *what, const void *p, uint
 KqTurns kq_turns(float theta, int neox, int hd);
 
 #ifdef __CUDACC__
-// cos and sin of pos * f turns.  The angle is reduced in 64 bits (in 32, the error of position 10^5 is 0.01); what the reduced
-// angle loses on its way to 32 bits is put back to first order.
-__device__ __forceinline__ float2 kq_turn(double f, int pos) {
-    double t = f * (double)pos;
-    t -= rint(t);
-    const float tf = (float)t, d = (float)(t - (double)tf) * 6.2831853f;
+// cos and sin of pos * f turns, f in units of 2^-64: the product's low 64 bits are the angle within its turn, to 2^-53 of f at least (in 32 bits the
+// error at position 10^5 would be 0.01).  Its first 24 bits are exact in f32, the next 24 are put back to first order.
+__device__ __forceinline__ float2 kq_turn(uint64_t f, int pos) {
+    const uint64_t x = f * (uint64_t)(uint32_t)pos;
+    const float t = (float)((int32_t)(x >> 32) >> 8) * 1.1920929e-7f /* 2^-23: half turns */, d = (float)((uint32_t)(x >> 16) & 0xffffffu) * (6.2831853f * 3.5527137e-15f /* 2^-48 */);
     float s, c;
-    sincospif(2.f * tf, &s, &c);
+    sincospif(t, &s, &c);
     return make_float2(fmaf(-s, d, c), fmaf(c, d, s));
 }
-// the same out of line, where it would be inlined many times over
-static __device__ __noinline__ float2 kq_turn_call(double f, int pos) { return kq_turn(f, pos); }
 // first and past-the-last row of sequence s, inside the call's rows whatever row_start holds
 __device__ __forceinline__ int2 kq_seq_rows(const KqBatch &b, int s) {
     const int lo = min(max(b.row_start[s], 0), b.rows), hi = min(max(b.row_start[s + 1], lo), b.rows);

@@ -223,7 +223,7 @@ KqTurns kq_turns(float theta, int neox, int hd) {
     t.neox = neox != 0;
     const double ratio = t.on ? pow((double)theta, -2.0 / hd) : 0.0; // one power: 63 products are off by 10^-14
     double f = t.on ? 1.0 / 6.283185307179586476925 : 0.0;
-    for (int i = 0; i < 64; i++, f *= ratio) t.f[i] = i < hd / 2 ? f : 0.0;
+    for (int i = 0; i < 64; i++, f *= ratio) t.f[i] = i < hd / 2 ? (uint64_t)(f * 18446744073709551616.0) : 0;
     return t;
 }
 

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
     __shared__ float sc_s[NW][NST][4];  // scales of the step's groups: keys, values
     __shared__ int have_s[NW][NST];     // which of them are there
     __shared__ float m_s[NW][R], l_s[NW][R];
-    __shared__ double turns_s[HD / 2]; // a lane's own entry is no broadcast: not from the constant bank
+    __shared__ uint64_t turns_s[HD / 2]; // a lane's own entry is no broadcast: not from the constant bank
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     if (tid < HD / 2) turns_s[tid] = a.turns.f[tid];
     uint8_t *ring = ring_s + warp * (NST * S::STEP);
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                     for (int i = 0; i < HD / 64; i++) {
                         const float v0 = x[2 * i], v1 = x[2 * i + 1];
                         if (a.turns.on) {
-                            const float2 cs = kq_turn_call(turns_s[lane + 32 * i], sq.pos(tok));
+                            const float2 cs = kq_turn(turns_s[lane + 32 * i], sq.pos(tok));
                             x[2 * i] = v0 * cs.x - v1 * cs.y;
                             x[2 * i + 1] = v0 * cs.y + v1 * cs.x;
                         }

@@ -90,6 +90,50 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// pairs of f32 in one register pair
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { // NaN if one is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t exp2_sfu(uint64_t x) {
+    const float2 v = unpack2(x);
+    return pack2(ex2(v.x), ex2(v.y));
+}
+// 2^x = 2^n 2^f, n the nearest whole number (added into the exponent), |f| <= 1/2: the cubic of least largest relative error there,
+// 7.5e-5 (a seventh of half a step of f16).  Below 2^-126 it gives next to nothing, as it should; a NaN is seen to with the maximum.
+constexpr int POLY = 3;
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+    const float2 v = unpack2(x);
+    x = pack2(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    const float magic = 12582912.f; // 1.5 * 2^23: adding it rounds to a whole number in the low bits
+    const uint64_t t = add2(x, pack2(magic, magic)), f = fma2(add2(t, pack2(-magic, -magic)), pack2(-1.f, -1.f), x);
+    uint64_t p = fma2(pack2(0.05517167f, 0.05517167f), f, pack2(0.24261114f, 0.24261114f));
+    p = fma2(p, f, pack2(0.69326097f, 0.69326097f));
+    p = fma2(p, f, pack2(0.99992806f, 0.99992806f));
+    const float2 tt = unpack2(t), pp = unpack2(p);
+    return pack2(__int_as_float(__float_as_int(pp.x) + (__float_as_int(tt.x) << 23)), __int_as_float(__float_as_int(pp.y) + (__float_as_int(tt.y) << 23)));
+}
 __device__ __forceinline__ uint32_t h2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -112,7 +156,7 @@ constexpr int MAX_SLOTS = 6;
 struct Shared {
     uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], raw_full[4], raw_empty[4], s_ready[2], p_ready[2], o_done, q_ready;
     float crow[R];
-    double turns[64]; // a lane's own entry is no broadcast: not from the constant bank
+    uint64_t turns[64]; // a lane's own entry is no broadcast: not from the constant bank
     uint32_t tmem;
     int abort;
 };
@@ -397,65 +441,80 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         uint32_t pieces = 0, units = 0;
         while (w.next(a)) {
             const int row0 = w.tile * R + 128 * half; // of this half, within the sequence and KV head
-            // ---- queries: a warp's 32 rows one after another, four rows' loads together; rows of one token share its angles
-            constexpr int P = HD / 64;
+            // ---- queries: a warp's 32 rows, eight at a time, the next eight's loads under way; rows of one token share its angles
+            constexpr int P = HD / 64, NB = 8;
             const bool split = a.turns.on && a.turns.neox;
-            int tok_cs = -1;
+            int tok = (row0 + (warp & 3) * 32) / a.G, h = row0 + (warp & 3) * 32 - tok * a.G; // of the next row
             float2 cs[P];
 #pragma unroll
             for (int u = 0; u < P; u++) cs[u] = make_float2(1.f, 0.f);
+            int tok_cs = -1;
             // the lane's pairs are P lane + u: dimensions (pair, pair + HD / 2) or (2 pair, 2 pair + 1)
-            int tok = (row0 + (warp & 3) * 32) / a.G, h = row0 + (warp & 3) * 32 - tok * a.G; // of the next row
-#pragma unroll 1
-            for (int rb = 0; rb < 32; rb += 4) {
-                float x[4][P][2];
-                int toks[4];
+            float2 nx[NB][P];
+            int ntok[NB];
+            auto fetch = [&](int k) { // row k of the next eight: elements 2 u, 2 u + 1 in the order they stand
+                ntok[k] = tok;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    toks[k] = tok;
+                for (int u = 0; u < P; u++) nx[k][u] = make_float2(0.f, 0.f);
+                if (tok < w.sq.t) {
+                    const T *q = (const T *)a.q + (int64_t)(w.sq.row0 + tok) * a.q_stride + (int64_t)(w.kh * a.G + h) * HD;
 #pragma unroll
-                    for (int u = 0; u < P; u++) x[k][u][0] = x[k][u][1] = 0.f;
-                    if (tok < w.sq.t) {
-                        const T *q = (const T *)a.q + (int64_t)(w.sq.row0 + tok) * a.q_stride + (int64_t)(w.kh * a.G + h) * HD;
-                        if (split && P == 2) {
-                            const float2 v0 = kq_ld2(q + 2 * lane), v1 = kq_ld2(q + HD / 2 + 2 * lane);
-                            x[k][0][0] = v0.x, x[k][P - 1][0] = v0.y, x[k][0][1] = v1.x, x[k][P - 1][1] = v1.y;
-                        } else if (split) {
-                            x[k][0][0] = kq_ld1(q + lane);
-                            x[k][0][1] = kq_ld1(q + HD / 2 + lane);
-                        } else {
-#pragma unroll
-                            for (int u = 0; u < P; u++) {
-                                const float2 v = kq_ld2(q + 2 * (P * lane + u));
-                                x[k][u][0] = v.x, x[k][u][1] = v.y;
-                            }
-                        }
-                    }
-                    if (++h == a.G) {
-                        h = 0;
-                        tok++;
+                    for (int u = 0; u < P; u++) {
+                        if (HD == 64 && split) nx[k][u] = make_float2(kq_ld1(q + lane), kq_ld1(q + HD / 2 + lane));
+                        else nx[k][u] = kq_ld2(q + (split ? u * (HD / 2) + 2 * lane : 2 * (P * lane + u)));
                     }
                 }
+                if (++h == a.G) {
+                    h = 0;
+                    tok++;
+                }
+            };
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int r = (warp & 3) * 32 + rb + k;
-                    if (a.turns.on && toks[k] != tok_cs && toks[k] < w.sq.t) {
-                        tok_cs = toks[k];
+            for (int k = 0; k < NB; k++) fetch(k);
+#pragma unroll 1
+            for (int rb = 0; rb < 32; rb += NB) {
+                float x[NB][P][2];
+                float2 c[NB][P];
 #pragma unroll
-                        for (int u = 0; u < P; u++) cs[u] = kq_turn_call(sh.turns[P * lane + u], w.sq.pos(tok_cs));
+                for (int k = 0; k < NB; k++) {
+                    if (a.turns.on && ntok[k] != tok_cs && ntok[k] < w.sq.t) {
+                        tok_cs = ntok[k];
+#pragma unroll
+                        for (int u = 0; u < P; u++) cs[u] = kq_turn(sh.turns[P * lane + u], w.sq.pos(tok_cs));
                     }
-                    float amax = 0.f;
+#pragma unroll
+                    for (int u = 0; u < P; u++) {
+                        c[k][u] = cs[u];
+                        if (split && P == 2) x[k][u][0] = u ? nx[k][0].y : nx[k][0].x, x[k][u][1] = u ? nx[k][P - 1].y : nx[k][P - 1].x;
+                        else x[k][u][0] = nx[k][u].x, x[k][u][1] = nx[k][u].y;
+                    }
+                }
+                if (rb + NB < 32) {
+#pragma unroll
+                    for (int k = 0; k < NB; k++) fetch(k);
+                }
+                float amax[NB];
+#pragma unroll
+                for (int k = 0; k < NB; k++) {
+                    amax[k] = 0.f;
 #pragma unroll
                     for (int u = 0; u < P; u++) {
                         const float v0 = x[k][u][0], v1 = x[k][u][1];
-                        x[k][u][0] = v0 * cs[u].x - v1 * cs[u].y;
-                        x[k][u][1] = v0 * cs[u].y + v1 * cs[u].x;
-                        amax = fmaxf(amax, fmaxf(fabsf(x[k][u][0]), fabsf(x[k][u][1])));
+                        x[k][u][0] = v0 * c[k][u].x - v1 * c[k][u].y;
+                        x[k][u][1] = v0 * c[k][u].y + v1 * c[k][u].x;
+                        amax[k] = fmaxf(amax[k], fmaxf(fabsf(x[k][u][0]), fabsf(x[k][u][1])));
                     }
-                    amax = kq_warp_max(amax);
-                    const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 252u);
-                    const float f = amax > 0.f ? __uint_as_float((254u - e) << 23) : 1.f;
-                    if (lane == 0) sh.crow[128 * half + r] = fmaxf(amax > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2, 1.2e-38f); // not 0: a hidden score times it is -inf
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int k = 0; k < NB; k++) amax[k] = fmaxf(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
+#pragma unroll
+                for (int k = 0; k < NB; k++) {
+                    const int r = (warp & 3) * 32 + rb + k;
+                    const uint32_t e = min(max(__float_as_uint(amax[k]) >> 23, 1u), 252u);
+                    const float f = amax[k] > 0.f ? __uint_as_float((254u - e) << 23) : 1.f;
+                    if (lane == 0) sh.crow[128 * half + r] = fmaxf(amax[k] > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2, 1.2e-38f); // not 0: a hidden score times it is -inf
                     auto put = [&](int d, float v0, float v1, bool two) { // dimension d (and d + 1)
 #pragma unroll
                         for (int p = 0; p < QS; p++) {
@@ -481,6 +540,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             arrive(smem_u32(&sh.q_ready));
             __syncwarp();
             const float crow = sh.crow[128 * half + row];
+            const bool my_row_ok = (row0 + row) / a.G < w.sq.t;
             const int my_tok = min((row0 + row) / a.G, w.sq.t - 1), lim = w.sq.p0 < 0 ? -1 : w.sq.pos(my_tok); // last position this row sees
             const int lim_lo = w.sq.pos(min(row0 / a.G, w.sq.t - 1)), lim_hi = w.sq.pos(min((row0 + 127) / a.G, w.sq.t - 1)); // of the half's rows
             const int seen = a.window > 0 ? max(0, w.sq.pos(w.tile * R / a.G) - a.window + 1) : 0;
@@ -540,7 +600,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         if (32 * c + j > last || 32 * c + j < first || !(blocks >> ((32 * c + j) >> 4) & 1)) s[j] = 0xff800000u; // -inf
                 };
                 uint32_t s[2][32];
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}; // a NaN stays: the whole row is NaN from there on
                 tmem_ld32(ts, s[0]);
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -548,12 +608,12 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     tmem_ld32(ts + 32 * ((c + 1) & 3), s[(c + 1) & 1]); // the last one begins the second reading
                     if (masked) mask(s[c & 1], c);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[c & 1][j]));
+                    for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(s[c & 1][j]), __uint_as_float(s[c & 1][j + 1]));
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * crow;
-                const bool grown = top > m + 8.f || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
+                const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * crow;
+                const bool grown = !(top <= m + 8.f) || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float mn = grown ? fmaxf(m, top) : m, alpha = mn == m ? 1.f : ex2(m - mn);
+                    const float mn = grown ? max3(m, top, top) : m, alpha = mn == m ? 1.f : ex2(m - mn);
                     m = mn;
                     if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                         l *= alpha;
@@ -569,8 +629,9 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     }
                 }
                 const float sub = m == -INFINITY ? 0.f : m - 6.f; // probabilities up to 2^14: small ones keep their bits in f16
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint64_t sums[2] = {0, 0};
                 uint32_t lo_even[PS == 2 ? 16 : 1];
+                const uint64_t crow2 = pack2(crow, crow), nsub2 = pack2(-sub, -sub);
                 // a chunk's probabilities go over scores that have been read: those of keys 0 .. 63 to columns 0 .. 31 (second parts 32 .. 63) ...
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
@@ -581,14 +642,21 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     uint32_t hi[16], lo[PS == 2 ? 16 : 1];
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
-                        const float p0 = ex2(fmaf(__uint_as_float(x[2 * j]), crow, -sub)), p1 = ex2(fmaf(__uint_as_float(x[2 * j + 1]), crow, -sub));
-                        sum[PS == 2 ? j >> 3 : j & 3] += p0 + p1;
-                        hi[j] = h2(p0, p1);
-                        if (PS == 2) lo[PS == 2 ? j : 0] = h2_low(p0, p1, hi[j]);
+                        uint64_t e = fma2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), crow2, nsub2);
+                        // results of 16 bits: 3 of 8 exponentials on the FMA pipe, so that neither it nor the special-function unit decides alone
+                        e = PS == 1 && j % 8 < POLY ? exp2_poly(e) : exp2_sfu(e);
+                        sums[PS == 2 ? j >> 3 : j & 1] = add2(sums[PS == 2 ? j >> 3 : j & 1], e);
+                        const float2 p = unpack2(e);
+                        hi[j] = h2(p.x, p.y);
+                        if (PS == 2) lo[PS == 2 ? j : 0] = h2_low(p.x, p.y, hi[j]);
                     }
                     if (PS == 2) {
-                        l = __fadd_rz(__fadd_rz(l, sum[0]), sum[1]);
-                        sum[0] = sum[1] = 0.f;
+#pragma unroll
+                        for (int g = 0; g < 2; g++) {
+                            const float2 v = unpack2(sums[g]);
+                            l = __fadd_rz(l, v.x + v.y);
+                            sums[g] = 0;
+                        }
                     }
                     if (PS == 2 && (c & 1) == 0) {
 #pragma unroll
@@ -603,7 +671,10 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     }
                 }
                 if (PS == 2) l = fmaf(l, -8.f * CUT_HALF_BIT, l); // the second parts' eight steps
-                else l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                else {
+                    const float2 v = unpack2(add2(sums[0], sums[1]));
+                    l += v.x + v.y;
+                }
                 if (!F8 && half == 0 && (key0 + BK > w.keys.y || key0 < seen)) {
                     // a value that no row sees may hold anything: it must not meet a probability of 0
                     const uint32_t v = 2 * units + 1;
@@ -623,12 +694,18 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             wait(sh.o_done, pieces & 1, 12);
             after_sync();
             if (PS == 2 && m_sum != -INFINITY) l = fmaf(l_sum, ex2(m_sum - m), l);
-            const bool whole = w.ub == 0 && w.take == w.n_units, ok = (row0 + row) / a.G < w.sq.t && !*abort;
-            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            const bool whole = w.ub == 0 && w.take == w.n_units, ok = my_row_ok && !*abort;
+            const float inv = m == -INFINITY ? 0.f : whole ? 1.f / l : 1.f; // a row that saw nothing is 0
             // 32 columns a time through the warp's part of the queries' room, so that a store writes whole lines of 4 rows
             uint8_t *turn = sm + half * L::TILE + (warp & 3) * 4096;
             const int cr = lane >> 3, cc = lane & 7; // row of four and 16-byte chunk of a store
-            const int wr0 = row0 + (warp & 3) * 32, wtok0 = wr0 / a.G, wh0 = wr0 - wtok0 * a.G;
+            int64_t to_row[8]; // where this lane's rows go, -1: nowhere
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int r = 4 * j + cr, rr = row0 + (warp & 3) * 32 + r, tok = rr / a.G, h = rr - tok * a.G; // r: of the warp's 32 rows
+                to_row[j] = tok >= w.sq.t || *abort ? -1 : whole ? (int64_t)(w.sq.row0 + tok) * a.out_stride + (int64_t)(w.kh * a.G + h) * HD + 4 * cc
+                                                        : (int64_t)slot * R * (HD + 2) + (int64_t)(128 * half + (warp & 3) * 32 + r) * HD + 4 * cc;
+            }
 #pragma unroll 1
             for (int k = 0; k < HD / 32; k++) {
                 uint32_t o[32];
@@ -638,23 +715,18 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 for (int j = 0; j < 8; j++) {
                     float4 v;
                     v.x = __uint_as_float(o[4 * j]) * inv, v.y = __uint_as_float(o[4 * j + 1]) * inv, v.z = __uint_as_float(o[4 * j + 2]) * inv, v.w = __uint_as_float(o[4 * j + 3]) * inv;
-                    if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (m == -INFINITY) v = make_float4(0.f, 0.f, 0.f, 0.f);
                     *reinterpret_cast<float4 *>(turn + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
                 }
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const int r = 4 * j + cr; // of the warp's 32 rows
+                    const int r = 4 * j + cr;
                     const float4 v = *reinterpret_cast<const float4 *>(turn + r * 128 + ((cc ^ (r & 7)) << 4));
-                    int tok = wtok0, h = wh0 + r;
-                    if (h >= a.G) {
-                        tok += h / a.G;
-                        h %= a.G;
-                    }
-                    if (tok >= w.sq.t || *abort) continue;
-                    if (!whole) *reinterpret_cast<float4 *>(a.part + (int64_t)slot * R * (HD + 2) + (int64_t)(128 * half + (warp & 3) * 32 + r) * HD + 32 * k + 4 * cc) = v;
+                    if (to_row[j] < 0) continue;
+                    if (!whole) *reinterpret_cast<float4 *>(a.part + to_row[j] + 32 * k) = v;
                     else {
-                        T *out = (T *)a.out + (int64_t)(w.sq.row0 + tok) * a.out_stride + (int64_t)(w.kh * a.G + h) * HD + 32 * k + 4 * cc;
+                        T *out = (T *)a.out + to_row[j] + 32 * k;
                         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out) = v;
                         else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<uint2 *>(out) = make_uint2(h2(v.x, v.y), h2(v.z, v.w));
                         else {
@@ -687,54 +759,61 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// joins the pieces of a split item: a warp per row, lanes the dimensions; grid (CTAs of the attention kernel, R / 16)
+// joins the pieces of a split item: a warp for two rows, lanes the dimensions, four pieces' loads together; grid (CTAs of the attention kernel, R / 16)
 template <int HD> __global__ void __launch_bounds__(256) pages_join_kernel(const __grid_constant__ KqAttnArgs a) {
     KQ_PDL_ENTER();
     const int4 meta = a.meta[2 * blockIdx.x], seq = a.meta[2 * blockIdx.x + 1];
     if (meta.x == 0) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r0 = blockIdx.y * 16 + 2 * warp;
+    if ((meta.z * R + r0) / a.G >= seq.y) return;
     constexpr int N = HD / 64;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float2 o[2][N];
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int u = 0; u < N; u++) o[k][u] = make_float2(0.f, 0.f);
+    for (int i0 = 0; i0 < meta.x; i0 += 4) {
+        float2 v[2][4][N];
+        float4 ml[4]; // of both rows
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int i = i0 + j;
+            ml[j] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+            const float *p = a.part + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * R * (HD + 2); // piece 0 is slot 2 b + 1, piece i slot 2 (b + i)
+            if (i < meta.x) ml[j] = *reinterpret_cast<const float4 *>(p + R * HD + 2 * r0);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int u = 0; u < N; u++) v[k][j][u] = i < meta.x ? *reinterpret_cast<const float2 *>(p + (r0 + k) * HD + 2 * (lane + 32 * u)) : make_float2(0.f, 0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            float mn = m[k];
+#pragma unroll
+            for (int j = 0; j < 4; j++) mn = fmaxf(mn, k ? ml[j].z : ml[j].x);
+            const float sub = mn == -INFINITY ? 0.f : mn, f0 = ex2(m[k] - sub);
+            l[k] *= f0;
+#pragma unroll
+            for (int u = 0; u < N; u++) o[k][u].x *= f0, o[k][u].y *= f0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float f = ex2((k ? ml[j].z : ml[j].x) - sub);
+                l[k] += f * (k ? ml[j].w : ml[j].y);
+#pragma unroll
+                for (int u = 0; u < N; u++) o[k][u].x += f * v[k][j][u].x, o[k][u].y += f * v[k][j][u].y;
+            }
+            m[k] = mn;
+        }
+    }
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const int r = blockIdx.y * 16 + 2 * warp + k, rr = meta.z * R + r, tok = rr / a.G;
+        const int rr = meta.z * R + r0 + k, tok = rr / a.G;
         if (tok >= seq.y) continue;
-        float m = -INFINITY, l = 0.f;
-        float2 o[N];
-#pragma unroll
-        for (int u = 0; u < N; u++) o[u] = make_float2(0.f, 0.f);
-        for (int i0 = 0; i0 < meta.x; i0 += 4) {
-            float2 ml[4], v[4][N];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int i = i0 + j;
-                ml[j] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-                for (int u = 0; u < N; u++) v[j][u] = make_float2(0.f, 0.f);
-                if (i < meta.x) { // piece 0 is slot 2 b + 1, piece i slot 2 (b + i)
-                    const float *p = a.part + (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * R * (HD + 2);
-                    ml[j] = *reinterpret_cast<const float2 *>(p + R * HD + 2 * r);
-#pragma unroll
-                    for (int u = 0; u < N; u++) v[j][u] = *reinterpret_cast<const float2 *>(p + r * HD + 2 * (lane + 32 * u));
-                }
-            }
-            const float mn = fmaxf(m, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x))), sub = mn == -INFINITY ? 0.f : mn;
-            const float f0 = ex2(m - sub);
-            l *= f0;
-#pragma unroll
-            for (int u = 0; u < N; u++) o[u].x *= f0, o[u].y *= f0;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float f = ex2(ml[j].x - sub);
-                l += f * ml[j].y;
-#pragma unroll
-                for (int u = 0; u < N; u++) o[u].x += f * v[j][u].x, o[u].y += f * v[j][u].y;
-            }
-            m = mn;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = l[k] == 0.f ? 0.f : 1.f / l[k];
 #pragma unroll
         for (int u = 0; u < N; u++)
-            kq_st2_type(a.type, a.out, (int64_t)(seq.x + tok) * a.out_stride + (int64_t)(meta.y * a.G + rr - tok * a.G) * HD + 2 * (lane + 32 * u), o[u].x * inv, o[u].y * inv);
+            kq_st2_type(a.type, a.out, (int64_t)(seq.x + tok) * a.out_stride + (int64_t)(meta.y * a.G + rr - tok * a.G) * HD + 2 * (lane + 32 * u), o[k][u].x * inv, o[k][u].y * inv);
     }
 }
 
