@@ -14,14 +14,12 @@
 // shared out evenly over one CTA per SM (kq_pages_sched.cuh).  Every wait is bounded: on a time-out the kernel records
 // an error, lets its copies land, frees its TMEM and returns.
 #include "kq_pages_sched.cuh"
+#include "kq_tc.cuh"
 
-#include <cuda.h>
 #include <math.h>
 #include <string.h>
 
 #include <type_traits>
-
-b200_status kq_tmap_encode(void *map128, int elem_bytes, int rank, const void *base, const uint64_t *dims, const uint64_t *strides_bytes, const uint32_t *box, int swizzle128);
 
 namespace {
 
@@ -36,52 +34,19 @@ constexpr float CUT_HALF_BIT = 4.3e-8f; // half a last bit relative to the value
 
 __device__ int g_pages_error;
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// shared-memory matrix descriptor, 128-byte swizzle
-__device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
 constexpr int HALF = BK * 128; // 128 rows of 64 dimensions
-// K-major operand (Q, K^T): rows of 128 bytes, groups of 8 rows 1024 bytes apart; step s of 16 dimensions
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int s) { return make_desc(tile + (s >> 2) * HALF + (s & 3) * 32, 16, 1024); }
-// MN-major operand (V): atoms of 64 dimensions HALF apart, groups of 8 positions 1024 bytes apart; step s of 16 positions
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int s) { return make_desc(tile + s * 2048, HALF, 1024); }
-__device__ __forceinline__ constexpr uint32_t idesc(bool b_mn, int n) { return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc) : "memory");
-}
-__device__ __forceinline__ void commit(uint32_t bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory"); }
+// steps of a product, in the address field of a descriptor (16 bytes): 16 dimensions of a K-major operand (Q, K^T), 16 positions of V
+__device__ __forceinline__ constexpr uint32_t step_k(int s) { return (s >> 2) * (HALF / 16) + (s & 3) * 2; }
+__device__ __forceinline__ constexpr uint32_t step_mn(int s) { return s * (2048 / 16); }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) { asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-                   "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-                 "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-                 "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-                 : "memory");
-}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t *r) { TMEM_LD32(taddr, r); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r) { TMEM_ST32(taddr, r); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) { TMEM_ST16(taddr, r); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -230,10 +195,6 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     uint8_t *sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     if (tid < HD / 2) sh.turns[tid] = a.turns.f[tid];
     if (tid == 0) {
         auto init = [](uint64_t &b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&b)), "r"(n)); };
@@ -254,20 +215,18 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.abort = 0;
     }
+    KQ_PDL_ENTER();
+    // behind the dependency wait: a CTA that starts early must not hold columns that its predecessor still has to allocate
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     before_sync();
     __syncthreads();
     after_sync();
     const uint32_t tmem = sh.tmem;
     volatile int *abort = &sh.abort;
-    auto wait = [&](uint64_t &bar, uint32_t parity, int code) {
-        for (int i = 0; i < 32; i++) // the clock is read only when it takes longer
-            if (kq_mbar_try(smem_u32(&bar), parity)) return;
-        if (!*abort && !kq_mbar_wait(smem_u32(&bar), parity, LIMIT)) {
-            *abort = 1;
-            atomicExch(&g_pages_error, code);
-        }
-    };
-    KQ_PDL_ENTER();
+    auto wait = [&](uint64_t &bar, uint32_t parity, int code) { return tc_wait(smem_u32(&bar), parity, abort, &g_pages_error, code, LIMIT); };
     const KqRun run = kq_find_run<R, BK, NT>(a);
     Walk w;
     w.start(a, run);
@@ -275,68 +234,84 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     int4 meta = make_int4(0, 0, 0, 0), meta2 = meta;
 
     if (warp == 8) {
-        // ---------------------------------------------------------------- products
-        if (lane == 0) {
-            uint32_t tile_n = 0, pieces = 0, units = 0; // ring tiles, pieces and units so far
-            while (w.next(a)) {
-                wait(sh.q_ready, pieces & 1, 1);
-                after_sync();
-                const uint32_t ring = smem_u32(sm + L::RING), q0 = smem_u32(sm);
-                auto slot = [&](uint32_t t) { return ring + (t % NS) * L::TILE; };
-                auto scores = [&](int half, uint32_t t) {
-                    if (*abort) return;
+        // ---------------------------------------------------------------- products: all lanes run the loop, one issues
+        const bool lead = tc_elect();
+        auto wait_all = [&](uint64_t &bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait(bar, parity, code)) != 0; };
+        const uint32_t ring = smem_u32(sm + L::RING);
+        const uint64_t dq = tc_desc(smem_u32(sm), 16, 1024), dk = tc_desc(ring, 16, 1024), dv = tc_desc(ring, HALF, 1024);
+        uint32_t pieces = 0, units = 0, ks = 0, kph = 0; // slot of the next tile of the ring and the parity of its round
+        bool ok = true;
+        auto scores = [&](int half, uint32_t slot) {
+            if (!lead || !ok) return;
+            const uint64_t b = dk + slot * (L::TILE / 16);
 #pragma unroll
-                    for (int p = 0; p < QS; p++)
+            for (int p = 0; p < QS; p++)
 #pragma unroll
-                        for (int s = 0; s < HD / 16; s++)
-                            mma_ss(tmem + COL_S + 128 * half, desc_k(q0 + (2 * p + half) * L::TILE, s), desc_k(slot(t), s), idesc(false, BK), p + s > 0);
-                };
-                auto values = [&](int half, uint32_t t, bool first) {
-                    if (*abort) return;
+                for (int s = 0; s < HD / 16; s++)
+                    tc_mma_ss(tmem + COL_S + 128 * half, dq + (2 * p + half) * (L::TILE / 16) + step_k(s), b + step_k(s), tc_idesc(128, BK, false, false), p + s > 0);
+        };
+        auto values = [&](int half, uint32_t slot, bool first) {
+            if (!lead || !ok) return;
+            const uint64_t b = dv + slot * (L::TILE / 16);
 #pragma unroll
-                    for (int p = 0; p < PS; p++)
+            for (int p = 0; p < PS; p++)
 #pragma unroll
-                        for (int s = 0; s < BK / 16; s++)
-                            mma_ts(tmem + COL_O + 128 * half, tmem + COL_S + 128 * half + 64 * (s >> 2) + 32 * p + 8 * (s & 3), desc_mn(slot(t), s), idesc(true, HD), !(first && p + s == 0));
-                };
-                wait(sh.full[tile_n % NS], (tile_n / NS) & 1, 2);
-                after_sync();
-                scores(0, tile_n);
-                commit(smem_u32(&sh.s_ready[0]));
-                scores(1, tile_n);
-                commit(smem_u32(&sh.s_ready[1]));
-                commit(smem_u32(&sh.empty[tile_n % NS]));
-                for (int i = 0; i < w.take; i++) {
-                    const uint32_t v = tile_n + 1, k = tile_n + 2;
-                    const bool more = i + 1 < w.take;
-                    wait(sh.p_ready[0], units & 1, 3);
-                    wait(sh.full[v % NS], (v / NS) & 1, 4);
-                    after_sync();
-                    values(0, v, PS == 2 ? i % FLUSH == 0 : i == 0);
-                    if (more) {
-                        wait(sh.full[k % NS], (k / NS) & 1, 5);
-                        after_sync();
-                        scores(0, k);
-                        commit(smem_u32(&sh.s_ready[0]));
-                    }
-                    wait(sh.p_ready[1], units & 1, 6);
-                    after_sync();
-                    values(1, v, PS == 2 ? i % FLUSH == 0 : i == 0);
-                    commit(smem_u32(&sh.empty[v % NS]));
-                    if (more) {
-                        scores(1, k);
-                        commit(smem_u32(&sh.s_ready[1]));
-                        commit(smem_u32(&sh.empty[k % NS]));
-                    }
-                    tile_n += 2;
-                    units++;
-                }
-                commit(smem_u32(&sh.o_done));
-                pieces++;
-                w.done();
+                for (int s = 0; s < BK / 16; s++)
+                    tc_mma_ts(tmem + COL_O + 128 * half, tmem + COL_S + 128 * half + 64 * (s >> 2) + 32 * p + 8 * (s & 3), b + step_mn(s), tc_idesc(128, HD, false, true),
+                              p + s > 0 ? 1u : first ? 0u : 1u);
+        };
+        auto next = [&](uint32_t &slot, uint32_t &ph) {
+            if (++slot == NS) slot = 0, ph ^= 1;
+        };
+        while (w.next(a)) {
+            ok = wait_all(sh.q_ready, pieces & 1, 1) && ok;
+            ok = wait_all(sh.full[ks], kph, 2) && ok;
+            after_sync();
+            scores(0, ks);
+            if (lead) tc_commit(smem_u32(&sh.s_ready[0]));
+            scores(1, ks);
+            if (lead) {
+                tc_commit(smem_u32(&sh.s_ready[1]));
+                tc_commit(smem_u32(&sh.empty[ks]));
             }
+            __syncwarp();
+            for (int i = 0; i < w.take; i++) {
+                const bool more = i + 1 < w.take, first = PS == 2 ? i % FLUSH == 0 : i == 0;
+                uint32_t vs = ks, vph = kph;
+                next(vs, vph);
+                ks = vs, kph = vph;
+                next(ks, kph);
+                ok = wait_all(sh.full[vs], vph, 4) && ok;
+                ok = wait_all(sh.p_ready[0], units & 1, 3) && ok;
+                after_sync();
+                values(0, vs, first);
+                __syncwarp();
+                if (more) {
+                    ok = wait_all(sh.full[ks], kph, 5) && ok;
+                    after_sync();
+                    scores(0, ks);
+                    if (lead) tc_commit(smem_u32(&sh.s_ready[0]));
+                    __syncwarp();
+                }
+                ok = wait_all(sh.p_ready[1], units & 1, 6) && ok;
+                after_sync();
+                values(1, vs, first);
+                if (lead) tc_commit(smem_u32(&sh.empty[vs]));
+                if (more) {
+                    scores(1, ks);
+                    if (lead) {
+                        tc_commit(smem_u32(&sh.s_ready[1]));
+                        tc_commit(smem_u32(&sh.empty[ks]));
+                    }
+                }
+                __syncwarp();
+                units++;
+            }
+            if (lead) tc_commit(smem_u32(&sh.o_done));
+            __syncwarp();
+            pieces++;
+            w.done();
         }
-        __syncwarp();
     } else if (warp == 9) {
         // ---------------------------------------------------------------- copies: a lane per box
         const int boxes = BK / box_rows, halves = F8 ? 1 : HD / 64, box = lane / halves, half = lane % halves;
