@@ -174,6 +174,10 @@ struct Walk {
     }
 };
 
+template <bool F8> __device__ __forceinline__ void less_registers() {
+    if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+}
 __device__ __noinline__ float2 turn_out_of_line(uint64_t f, int pos) { return kq_turn(f, pos); }
 // codes of 8 dimensions as f16 numbers times the block's scale
 __device__ __forceinline__ uint4 decode8(uint32_t lo, uint32_t hi, __half2 s) {
@@ -235,7 +239,9 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     const int bpp = a.c.page / KQ_PAGE_BLOCK;
     int4 meta = make_int4(0, 0, 0, 0), meta2 = meta;
 
+    // registers: the launch's 384 x 168 as 256 x 208 + 128 x 88, or 512 x 128 as 256 x 184 + 256 x 72
     if (warp == 8) {
+        less_registers<F8>();
         // ---------------------------------------------------------------- products: all lanes run the loop, one issues
         const bool lead = tc_elect();
         auto wait_all = [&](uint64_t &bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, wait(bar, parity, code)) != 0; };
@@ -317,6 +323,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             w.done();
         }
     } else if (warp == 9) {
+        less_registers<F8>();
         // ---------------------------------------------------------------- copies: a lane per box
         const int boxes = BK / box_rows, halves = F8 ? 1 : HD / 64, box = lane / halves, half = lane % halves;
         uint32_t tile_n = 0;
@@ -366,6 +373,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             }
         __syncwarp();
     } else if (F8 && warp >= 12) {
+        less_registers<F8>();
         // ---------------------------------------------------------------- e4m3 rows to the f16 tile: a thread per position
         const int c = tid - 384;
         uint32_t tile_n = 0;
@@ -414,6 +422,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             w.done();
         }
     } else if (warp < 8) {
+        if (F8) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         // ---------------------------------------------------------------- queries, softmax, results: a thread per row
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + COL_S + 128 * half, to = tl + COL_O + 128 * half;
@@ -430,14 +440,17 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 const int b = c >> 3, part = HD == 128 ? b >> 1 : b;
                 return sm + (2 * part + half) * L::TILE + (HD == 128 ? (b & 1) * HALF : 0) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
             };
+            {
+                constexpr int STEP = 32 / CH; // rows of one copy of the warp
+                int ctok = tok0, ch = h0 + lane / CH;
+                const int c = lane % CH;
 #pragma unroll 4
-            for (int i = lane; i < 32 * CH; i += 32) {
-                const int r = i / CH, c = i % CH;
-                int tok = tok0, h = h0 + r;
-                if (h >= a.G) tok += h / a.G, h %= a.G;
-                const bool there = tok < w.sq.t;
-                const T *src = (const T *)a.q + (there ? (int64_t)(w.sq.row0 + tok) * a.q_stride + (int64_t)(w.kh * a.G + h) * HD + c * (16 / (int)sizeof(T)) : 0);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(raw_at(wrow + r, c))), "l"(src), "r"(there ? 16 : 0) : "memory");
+                for (int r = lane / CH; r < 32; r += STEP, ch += STEP) {
+                    while (ch >= a.G) ch -= a.G, ctok++;
+                    const bool there = ctok < w.sq.t;
+                    const T *src = (const T *)a.q + (there ? (int64_t)(w.sq.row0 + ctok) * a.q_stride + (int64_t)(w.kh * a.G + ch) * HD + c * (16 / (int)sizeof(T)) : 0);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(raw_at(wrow + r, c))), "l"(src), "r"(there ? 16 : 0) : "memory");
+                }
             }
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
             __syncwarp();
@@ -584,7 +597,6 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     l = 0.f;
                     m_sum = m;
                 }
-                // the scores are read twice, 32 at a time (the maximum, then the probabilities): a row of 128 would not fit next to the rest
                 const bool masked = blocks != 0xff || key0 + BK - 1 > lim_lo || (a.window > 0 && key0 <= lim_hi - a.window);
                 const int last = lim - key0, first = a.window > 0 ? last - a.window + 1 : -0x40000000;
                 auto mask = [&](uint32_t *s, int c) {
@@ -598,20 +610,19 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     for (int j = 0; j < 32; j++)
                         if (!(see >> j & 1)) s[j] = 0xff800000u; // -inf
                 };
-                uint32_t s[2][32];
+                uint32_t s[4][32];
                 float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}; // a NaN stays: the whole row is NaN from there on
-                tmem_ld32(ts, s[0]);
-#pragma unroll 1
-                for (int x = 0; x < 2; x++) // (these loops stay loops: their code is large)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int c = 2 * x + e;
-                        tmem_ld_wait();
-                        tmem_ld32(ts + 32 * ((c + 1) & 3), s[e ^ 1]); // the last one begins the second reading
-                        if (masked) mask(s[e], c);
+                for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, s[c]);
+                tmem_ld_wait();
+                if (masked) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(s[e][j]), __uint_as_float(s[e][j + 1]));
-                    }
+                    for (int c = 0; c < 4; c++) mask(s[c], c);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1]));
                 const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * crow;
                 const bool grown = !(top <= m + 8.f) || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
                 if (__any_sync(0xffffffffu, grown)) {
@@ -646,16 +657,13 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 uint32_t lo_even[PS == 2 ? 16 : 1];
                 const uint64_t crow2 = pack2(crow, crow), nsub2 = pack2(-sub, -sub);
                 // a chunk's probabilities go over scores that have been read: those of keys 0 .. 63 to columns 0 .. 31 (second parts 32 .. 63) ...
-#pragma unroll 1
+#pragma unroll
                 for (int h64 = 0; h64 < 2; h64++) {
                     uint32_t hi[16], lo[PS == 2 ? 16 : 1];
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int c = 2 * h64 + e;
-                        tmem_ld_wait();
-                        if (c < 3) tmem_ld32(ts + 32 * (c + 1), s[e ^ 1]);
-                        uint32_t(&x)[32] = s[e];
-                        if (masked) mask(x, c);
+                        uint32_t(&x)[32] = s[c];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
                             uint64_t v = fma2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), crow2, nsub2);
@@ -760,7 +768,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             a.meta[2 * blockIdx.x] = meta;
             a.meta[2 * blockIdx.x + 1] = meta2;
         }
-    }
+    } else less_registers<F8>();
     before_sync();
     __syncthreads();
     if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
