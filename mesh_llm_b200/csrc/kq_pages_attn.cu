@@ -5,7 +5,7 @@
 // From there the fragments of mma.m16n8k16 are 16-byte reads: the order of a product's inner index is free, so the 16 bytes that a thread reads of a
 // key are the dimensions that its lane holds in consecutive steps of Q K^T, and Q is laid out to match; of the values it
 // reads 16 bytes of four keys and pairs them up by byte permutes into the rows of V^T.  16-byte chunks are stored at chunk ^ (row % 8), which keeps both
-// kinds of read off each other's banks.  e4m3 codes become f16 in registers (K's scale goes onto the score, V's onto the value, both
+// kinds of read off each other's banks.  e4m3 codes become f16 in registers (K's scale goes onto the score, V's onto the product, both
 // exact powers of two).  Scores are Q K^T with the item's rows as the 16 rows of the tile; the probabilities are then already the
 // B operand of O^T = V^T P^T.  Softmax in base 2, statistics in 32 bits.
 // A query row enters divided by the power of two that brings its largest element to [1, 2), so f16 neither overflows nor loses small
@@ -48,10 +48,6 @@ __device__ __forceinline__ uint32_t h2_low(float a, float b, uint32_t hi) { // w
     const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
     return h2(a - f.x, b - f.y);
 }
-__device__ __forceinline__ uint32_t mul_h2(uint32_t a, __half2 b) {
-    const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&a), b);
-    return *reinterpret_cast<const uint32_t *>(&r);
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -61,8 +57,11 @@ __device__ __forceinline__ float ex2(float x) {
 template <int HD, bool F8, int HT> struct Shape {
     static constexpr int R = 8 * HT, ES = F8 ? 1 : 2, ROW = HD * ES, NG = F8 ? 2 : 1, KT = 16 * NG; // groups of 16 positions of a warp's step
     static constexpr int STEP = 2 * KT * ROW;                                                       // keys, then values
-    static constexpr int NST = STEP == 8192 ? (HT == 1 ? 2 : 3) : 4;                                // ring stages of a warp
-    static constexpr int CTAS = HT == 1 ? 3 : 2;                                                    // per SM
+    #ifndef DV
+#define DV 0
+#endif
+    static constexpr int NST = STEP == 8192 ? (HT == 1 && DV != 1 ? 2 : 3) : 4;                                // ring stages of a warp
+    static constexpr int CTAS = HT == 1 && DV != 1 ? 3 : 2;                                                    // per SM
     static constexpr int SMEM = NW * NST * STEP;
     static_assert(NST * STEP >= R * HD * 4, "a warp's rows fit into its ring");
 };
@@ -198,23 +197,25 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                     if (lane == 0) c_s[r] = amax > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2;
                 }
                 __syncthreads();
-                uint32_t qh[KS][4], ql[SPLIT ? KS : 1][4];
+                // Q as the A operand: rows g and g + 8 of the tile.  Up to 8 rows: the second parts take the other 8 places of the same product.
+                uint32_t qh[KS][4], ql[SPLIT && HT == 2 ? KS : 1][4];
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     const int d = F8 ? 64 * (ks >> 2) + 16 * t4 + 4 * (ks & 3) : 32 * (ks >> 1) + 8 * t4 + 4 * (ks & 1);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (h >= HT) {
-                            qh[ks][h] = qh[ks][h + 2] = 0u;
-                            if (SPLIT) ql[ks][h] = ql[ks][h + 2] = 0u;
-                            continue;
-                        }
-                        const float4 v = *reinterpret_cast<const float4 *>(&q_s[g + 8 * h][d]);
-                        qh[ks][h] = h2(v.x, v.y);
-                        qh[ks][h + 2] = h2(v.z, v.w);
-                        if (SPLIT) {
-                            ql[ks][h] = h2_low(v.x, v.y, qh[ks][h]);
-                            ql[ks][h + 2] = h2_low(v.z, v.w, qh[ks][h + 2]);
+                        const float4 v = *reinterpret_cast<const float4 *>(&q_s[g + (HT == 2 ? 8 * h : 0)][d]);
+                        const uint32_t x = h2(v.x, v.y), y = h2(v.z, v.w);
+                        if (HT == 2 || h == 0) {
+                            qh[ks][h] = x;
+                            qh[ks][h + 2] = y;
+                            if (SPLIT && HT == 2) {
+                                ql[SPLIT && HT == 2 ? ks : 0][h] = h2_low(v.x, v.y, x);
+                                ql[SPLIT && HT == 2 ? ks : 0][h + 2] = h2_low(v.z, v.w, y);
+                            }
+                        } else {
+                            qh[ks][h] = SPLIT ? h2_low(v.x, v.y, x) : 0u;
+                            qh[ks][h + 2] = SPLIT ? h2_low(v.z, v.w, y) : 0u;
                         }
                     }
                 }
@@ -255,8 +256,12 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                                     const uint32_t b0 = F8 ? kq_e4m3x2_h2((uint16_t)word(kr, x)) : word(kr, 2 * x);
                                     const uint32_t b1 = F8 ? kq_e4m3x2_h2((uint16_t)(word(kr, x) >> 16)) : word(kr, 2 * x + 1);
                                     mma(c, qh[ks], b0, b1);
-                                    if (SPLIT) mma(c, ql[SPLIT ? ks : 0], b0, b1);
+                                    if (SPLIT && HT == 2) mma(c, ql[SPLIT && HT == 2 ? ks : 0], b0, b1);
                                 }
+                            }
+                            if (SPLIT && HT == 1) {
+                                c[0] += c[2];
+                                c[1] += c[3];
                             }
                         }
                     float mx[HT];
@@ -335,14 +340,11 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                                 for (int j = 0; j < VL; j++) vr[n][x][j] = *reinterpret_cast<const uint4 *>(vst + place<ROW>(r, 8 * j + g));
                             }
                         }
-                    __half2 vs2[NG];
+                    float vsc[NG]; // a group's scale goes onto its product, exactly
 #pragma unroll
-                    for (int n = 0; n < NG; n++) vs2[n] = __float2half2_rn(F8 && (have >> n & 1) ? sc_s[warp][st][2 + n] : 0.f);
+                    for (int n = 0; n < NG; n++) vsc[n] = F8 && (have >> n & 1) ? sc_s[warp][st][2 + n] : 0.f;
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
-                        float part[HT][4];
-#pragma unroll
-                        for (int h = 0; h < HT; h++) part[h][0] = part[h][1] = part[h][2] = part[h][3] = 0.f;
 #pragma unroll
                         for (int n = 0; n < NG; n++) {
                             uint32_t va[4];
@@ -350,10 +352,10 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                                 const uint32_t pick = i & 1 ? 0x7362u : 0x5140u;
                                 const uint32_t x = __byte_perm(word(vr[n][0][0], i >> 1), word(vr[n][1][0], i >> 1), pick);
                                 const uint32_t y = __byte_perm(word(vr[n][2][0], i >> 1), word(vr[n][3][0], i >> 1), pick);
-                                va[0] = mul_h2(kq_e4m3x2_h2((uint16_t)x), vs2[n]);
-                                va[1] = mul_h2(kq_e4m3x2_h2((uint16_t)(x >> 16)), vs2[n]);
-                                va[2] = mul_h2(kq_e4m3x2_h2((uint16_t)y), vs2[n]);
-                                va[3] = mul_h2(kq_e4m3x2_h2((uint16_t)(y >> 16)), vs2[n]);
+                                va[0] = kq_e4m3x2_h2((uint16_t)x);
+                                va[1] = kq_e4m3x2_h2((uint16_t)(x >> 16));
+                                va[2] = kq_e4m3x2_h2((uint16_t)y);
+                                va[3] = kq_e4m3x2_h2((uint16_t)(y >> 16));
                             } else {
                                 const uint32_t w0 = word(vr[n][0][i >> 2], i & 3), w1 = word(vr[n][1][i >> 2], i & 3);
                                 const uint32_t w2 = word(vr[n][2][i >> 2], i & 3), w3 = word(vr[n][3][i >> 2], i & 3);
@@ -364,17 +366,16 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                             }
 #pragma unroll
                             for (int h = 0; h < HT; h++) {
-                                if (SPLIT) {
-                                    mma(part[h], va, pl[SPLIT ? n : 0][h][0], pl[SPLIT ? n : 0][h][1]);
-                                    mma(part[h], va, ph[n][h][0], ph[n][h][1]);
-                                } else mma(o[h][i], va, ph[n][h][0], ph[n][h][1]);
+                                if (!SPLIT && !F8) {
+                                    mma(o[h][i], va, ph[n][h][0], ph[n][h][1]);
+                                    continue;
+                                }
+                                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                                if (SPLIT) mma(part, va, pl[SPLIT ? n : 0][h][0], pl[SPLIT ? n : 0][h][1]);
+                                mma(part, va, ph[n][h][0], ph[n][h][1]);
+#pragma unroll
+                                for (int x = 0; x < 4; x++) o[h][i][x] = F8 ? fmaf(part[x], vsc[n], o[h][i][x]) : o[h][i][x] + part[x];
                             }
-                        }
-                        if (SPLIT) {
-#pragma unroll
-                            for (int h = 0; h < HT; h++)
-#pragma unroll
-                                for (int x = 0; x < 4; x++) o[h][i][x] += part[h][x];
                         }
                     }
                 }
