@@ -57,16 +57,15 @@ __device__ __forceinline__ float ex2(float x) {
 template <int HD, bool F8, int HT> struct Shape {
     static constexpr int R = 8 * HT, ES = F8 ? 1 : 2, ROW = HD * ES, NG = F8 ? 2 : 1, KT = 16 * NG; // groups of 16 positions of a warp's step
     static constexpr int STEP = 2 * KT * ROW;                                                       // keys, then values
-    #ifndef DV
-#define DV 0
-#endif
-    static constexpr int NST = STEP == 8192 ? (HT == 1 && DV != 1 ? 2 : 3) : 4;                                // ring stages of a warp
-    static constexpr int CTAS = HT == 1 && DV != 1 ? 3 : 2;                                                    // per SM
+        static constexpr int NST = STEP == 8192 ? (HT == 1 ? 2 : 3) : 4; // ring stages of a warp
+    static constexpr int CTAS = HT == 1 ? 3 : 2;                     // per SM (2 of 3 stages each: 64 sequences 79 us instead of 75, 200 in 8 bits 208 instead of 188)
     static constexpr int SMEM = NW * NST * STEP;
     static_assert(NST * STEP >= R * HD * 4, "a warp's rows fit into its ring");
 };
 // place of 16-byte chunk c of row r
 template <int ROW> __device__ __forceinline__ int place(int r, int c) { return r * ROW + ((c ^ (ROW >= 128 ? r & 7 : (r >> 1) & 3)) << 4); }
+
+__device__ __noinline__ float2 turn_out_of_line(uint64_t f, int pos) { return kq_turn(f, pos); }
 
 // HT: tiles of 8 rows (1 or 2); T: the activations' type, all but bf16 (whose results have 8 bits) with queries and probabilities in two f16 parts
 template <int HD, bool F8, int HT, typename T>
@@ -101,7 +100,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
         int kh = (int)kq_div(run.off, per_head), tile = 0;
         long long uo = run.off - kh * per_head;
         while (tile < tiles) { // the tile that the run begins in
-            const int n = kq_units<U>(kq_tile_keys<R>(a, sq, tile));
+            const int n = kq_units<U>(kq_tile_keys<R>(a, sq, tile)) + kq_setup<R>;
             if (uo < n) break;
             uo -= n;
             tile++;
@@ -109,8 +108,26 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
         for (; kh < a.c.n_kv && u < run.u1; kh++, tile = 0)
             for (; tile < tiles && u < run.u1; tile++, uo = 0) {
                 const int2 keys = kq_tile_keys<R>(a, sq, tile);
-                const int n_units = kq_units<U>(keys), take = (int)min((long long)n_units - uo, run.u1 - u), ub = (int)uo;
-                u += take;
+                const int n_units = kq_units<U>(keys), part = (int)min((long long)n_units + kq_setup<R> - uo, run.u1 - u);
+                const int ub = max(0, (int)uo - kq_setup<R>), take = max(0, (int)uo + part - kq_setup<R>) - ub;
+                u += part;
+                if (take == 0) continue; // the next CTA's
+                // the queries' loads, under way while the positions are asked for
+                float x[R / NW][HD / 32];
+                int qtok[R / NW];
+#pragma unroll
+                for (int y = 0; y < R / NW; y++) {
+                    const int rr = tile * R + warp + NW * y, tok = rr / a.G, h = kh * a.G + rr - tok * a.G;
+                    const bool ok = tok < sq.t;
+                    qtok[y] = tok;
+                    const T *row = (const T *)a.q + (int64_t)(sq.row0 + (ok ? tok : 0)) * a.q_stride + (int64_t)(ok ? h : 0) * HD;
+#pragma unroll
+                    for (int i = 0; i < HD / 64; i++) {
+                        const int pr = lane + 32 * i;
+                        x[y][2 * i] = ok ? kq_ld1(row + (a.turns.neox ? pr : 2 * pr)) : 0.f;
+                        x[y][2 * i + 1] = ok ? kq_ld1(row + (a.turns.neox ? pr + HD / 2 : 2 * pr + 1)) : 0.f;
+                    }
+                }
                 __syncthreads(); // the item before has been joined
                 const int bpp = a.c.page / KQ_PAGE_BLOCK;
                 const int64_t head_off = (int64_t)kh * a.c.page * ROW;
@@ -162,28 +179,19 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                 };
                 for (int i = 0; i < NST - 1; i++) ask(i);
                 // ---- the item's queries: rotated, normed, in shared memory
-#pragma unroll 1
-                for (int r = warp; r < R; r += NW) {
-                    const int rr = tile * R + r, tok = rr / a.G, h = kh * a.G + rr - tok * a.G;
-                    const bool ok = tok < sq.t;
-                    const T *row = (const T *)a.q + (int64_t)(sq.row0 + (ok ? tok : 0)) * a.q_stride + (int64_t)(ok ? h : 0) * HD;
-                    float x[HD / 32];
 #pragma unroll
-                    for (int i = 0; i < HD / 64; i++) {
-                        const int pr = lane + 32 * i;
-                        x[2 * i] = ok ? kq_ld1(row + (a.turns.neox ? pr : 2 * pr)) : 0.f;
-                        x[2 * i + 1] = ok ? kq_ld1(row + (a.turns.neox ? pr + HD / 2 : 2 * pr + 1)) : 0.f;
-                    }
+                for (int y = 0; y < R / NW; y++) {
+                    const int r = warp + NW * y;
                     float amax = 0.f;
 #pragma unroll
                     for (int i = 0; i < HD / 64; i++) {
-                        const float v0 = x[2 * i], v1 = x[2 * i + 1];
+                        const float v0 = x[y][2 * i], v1 = x[y][2 * i + 1];
                         if (a.turns.on) {
-                            const float2 cs = kq_turn(turns_s[lane + 32 * i], sq.pos(tok));
-                            x[2 * i] = v0 * cs.x - v1 * cs.y;
-                            x[2 * i + 1] = v0 * cs.y + v1 * cs.x;
+                            const float2 cs = turn_out_of_line(turns_s[lane + 32 * i], sq.pos(qtok[y]));
+                            x[y][2 * i] = v0 * cs.x - v1 * cs.y;
+                            x[y][2 * i + 1] = v0 * cs.y + v1 * cs.x;
                         }
-                        amax = fmaxf(amax, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
+                        amax = fmaxf(amax, fmaxf(fabsf(x[y][2 * i]), fabsf(x[y][2 * i + 1])));
                     }
                     amax = kq_warp_max(amax);
                     const uint32_t e = min(max(__float_as_uint(amax) >> 23, 1u), 252u);
@@ -191,8 +199,8 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
 #pragma unroll
                     for (int i = 0; i < HD / 64; i++) {
                         const int pr = lane + 32 * i;
-                        q_s[r][a.turns.neox ? pr : 2 * pr] = x[2 * i] * f;
-                        q_s[r][a.turns.neox ? pr + HD / 2 : 2 * pr + 1] = x[2 * i + 1] * f;
+                        q_s[r][a.turns.neox ? pr : 2 * pr] = x[y][2 * i] * f;
+                        q_s[r][a.turns.neox ? pr + HD / 2 : 2 * pr + 1] = x[y][2 * i + 1] * f;
                     }
                     if (lane == 0) c_s[r] = amax > 0.f ? a.scale_log2 * __uint_as_float(e << 23) : a.scale_log2;
                 }
@@ -406,29 +414,43 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                     meta = make_int4(1 + (n_units - take + per - 1) / per, kh, tile, 0);
                     meta2 = make_int4(sq.row0, sq.t, 0, 0);
                 }
-                for (int i = tid; i < R * (HD / 2); i += NT) {
-                    const int r = i / (HD / 2), d = 2 * (i % (HD / 2));
-                    const int rr = tile * R + r, tok = rr / a.G;
+                constexpr int TR = 16, PER = HD / TR; // threads of a row, dimensions of a thread
+#pragma unroll 1
+                for (int r = tid / TR; r < R; r += NT / TR) {
+                    const int rr = tile * R + r, tok = rr / a.G, d0 = (tid % TR) * 4;
                     if (tok >= sq.t) continue;
-                    float mm = m_s[0][r];
+                    float mm = m_s[0][r], ll = 0.f, v[PER];
 #pragma unroll
                     for (int w = 1; w < NW; w++) mm = fmaxf(mm, m_s[w][r]);
                     const float sub = mm == -INFINITY ? 0.f : mm;
-                    float x = 0.f, y = 0.f, ll = 0.f;
+#pragma unroll
+                    for (int k = 0; k < PER; k++) v[k] = 0.f;
 #pragma unroll
                     for (int w = 0; w < NW; w++) {
                         const float f = ex2(m_s[w][r] - sub);
-                        const float2 v = *reinterpret_cast<const float2 *>(&o_at(w)[r][d]);
-                        x += f * v.x;
-                        y += f * v.y;
                         ll += f * l_s[w][r];
+#pragma unroll
+                        for (int k = 0; k < PER; k += 4) { // dimensions d0 + 16 k ..
+                            const float4 y = *reinterpret_cast<const float4 *>(&o_at(w)[r][d0 + 16 * k]);
+                            v[k] += f * y.x, v[k + 1] += f * y.y, v[k + 2] += f * y.z, v[k + 3] += f * y.w;
+                        }
                     }
                     if (whole) {
                         const float inv = ll == 0.f ? 0.f : 1.f / ll;
-                        kq_st2_type(a.type, a.out, (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(kh * a.G + rr % a.G) * HD + d, x * inv, y * inv);
+                        T *out = (T *)a.out + (int64_t)(sq.row0 + tok) * a.out_stride + (int64_t)(kh * a.G + rr - tok * a.G) * HD + d0;
+#pragma unroll
+                        for (int k = 0; k < PER; k += 4) {
+                            if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out + 16 * k) = make_float4(v[k] * inv, v[k + 1] * inv, v[k + 2] * inv, v[k + 3] * inv);
+                            else if constexpr (SPLIT) *reinterpret_cast<uint2 *>(out + 16 * k) = make_uint2(h2(v[k] * inv, v[k + 1] * inv), h2(v[k + 2] * inv, v[k + 3] * inv));
+                            else {
+                                const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v[k] * inv, v[k + 1] * inv), __floats2bfloat162_rn(v[k + 2] * inv, v[k + 3] * inv)};
+                                *reinterpret_cast<uint2 *>(out + 16 * k) = *reinterpret_cast<const uint2 *>(b);
+                            }
+                        }
                     } else {
-                        *reinterpret_cast<float2 *>(po + r * HD + d) = make_float2(x, y);
-                        if (d == 0) *reinterpret_cast<float2 *>(pml + 2 * r) = make_float2(mm, ll);
+#pragma unroll
+                        for (int k = 0; k < PER; k += 4) *reinterpret_cast<float4 *>(po + r * HD + d0 + 16 * k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                        if (d0 == 0) *reinterpret_cast<float2 *>(pml + 2 * r) = make_float2(mm, ll);
                     }
                 }
             }

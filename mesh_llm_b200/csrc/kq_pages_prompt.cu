@@ -142,31 +142,34 @@ struct Walk {
         uo = run.off - kh * run.per_head;
         tiles = kq_tiles<R>(a, sq.t);
         for (tile = 0;; tile++) {
-            n_units = kq_units<BK>(kq_tile_keys<R>(a, sq, tile));
-            if (uo < n_units || tile + 1 >= tiles) break;
-            uo -= n_units;
+            const int n = kq_units<BK>(kq_tile_keys<R>(a, sq, tile)) + kq_setup<R>;
+            if (uo < n || tile + 1 >= tiles) break;
+            uo -= n;
         }
     }
     // the next piece; false: no more
     __device__ bool next(const KqAttnArgs &a) {
-        if (u >= u1) return false;
-        while (tile >= tiles) {
-            tile = 0;
-            if (++kh >= a.c.n_kv) {
-                kh = 0;
-                do {
-                    if (++s >= a.b.n_seq) return false;
-                    sq = kq_seq(a, s);
-                } while (sq.t == 0);
-                tiles = kq_tiles<R>(a, sq.t);
+        for (;; done()) {
+            if (u >= u1) return false;
+            while (tile >= tiles) {
+                tile = 0;
+                if (++kh >= a.c.n_kv) {
+                    kh = 0;
+                    do {
+                        if (++s >= a.b.n_seq) return false;
+                        sq = kq_seq(a, s);
+                    } while (sq.t == 0);
+                    tiles = kq_tiles<R>(a, sq.t);
+                }
             }
+            keys = kq_tile_keys<R>(a, sq, tile);
+            n_units = kq_units<BK>(keys);
+            const int part = (int)min((long long)n_units + kq_setup<R> - uo, u1 - u);
+            ub = max(0, (int)uo - kq_setup<R>);
+            take = max(0, (int)uo + part - kq_setup<R>) - ub;
+            u += part;
+            if (take > 0) return true; // else the item is the next CTA's
         }
-        keys = kq_tile_keys<R>(a, sq, tile);
-        n_units = kq_units<BK>(keys);
-        take = (int)min((long long)n_units - uo, u1 - u);
-        ub = (int)uo;
-        u += take;
-        return true;
     }
     __device__ void done() {
         tile++;

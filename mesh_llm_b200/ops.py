@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 
 import torch
 
@@ -280,79 +281,94 @@ def kv_pages(n_pages, page_size, n_kv, hd, dtype=torch.float16, device="cuda"):
 
 def _pages_call(rows, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale):
     """the C descriptors of a paged cache and a batch, checked against one another"""
-    type_ = _PAGE_TYPES.get(k_pages.dtype)
-    if type_ is None or v_pages.dtype != k_pages.dtype:
-        raise ValueError(f"pages of {k_pages.dtype} / {v_pages.dtype}: float16 or float8_e4m3fn expected")
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.stride() != k_pages.stride():
+    dtype, shape, stride = k_pages.dtype, k_pages.shape, k_pages.stride()
+    type_ = _PAGE_TYPES.get(dtype)
+    if type_ is None or v_pages.dtype is not dtype:
+        raise ValueError(f"pages of {dtype} / {v_pages.dtype}: float16 or float8_e4m3fn expected")
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride:
         raise ValueError("pages: two pools [n_pages, n_kv, page_size, hd] of one shape and layout expected")
-    n_pages, n_kv, size, hd = k_pages.shape
-    stride = k_pages.stride()
+    n_pages, n_kv, size, hd = shape
     if n_pages and stride[1:] != (size * hd, hd, 1):
         raise ValueError("pages: each page must be contiguous")
+    dev = rows.get_device()
     if type_ == TYPE_F8_E4M3:
         for s in (k_scale, v_scale):
-            if s is None or s.dtype != torch.float32 or s.shape != (n_pages, n_kv, size // 16) or not s.is_contiguous():
-                raise ValueError("pages of float8_e4m3fn need k_scale and v_scale: contiguous f32 [n_pages, n_kv, page_size // 16]")
+            if s is None or s.dtype is not torch.float32 or s.shape != (n_pages, n_kv, size // 16) or not s.is_contiguous() or s.get_device() != dev:
+                raise ValueError("pages of float8_e4m3fn need k_scale and v_scale on their device: contiguous f32 [n_pages, n_kv, page_size // 16]")
+        scales = k_scale.data_ptr(), v_scale.data_ptr()
+    else:
+        scales = None, None
     n_seq = pos0.numel()
-    for name, t, n in (("pos0", pos0, n_seq), ("row_start", row_start, n_seq + 1)):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name}: contiguous int32 [{n}] expected")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != n_seq or (table.shape[1] > 1 and table.stride(1) != 1):
+    if pos0.dtype is not torch.int32 or pos0.dim() != 1 or not pos0.is_contiguous():
+        raise ValueError("pos0: contiguous int32 [sequences] expected")
+    if row_start.dtype is not torch.int32 or row_start.shape != (n_seq + 1,) or not row_start.is_contiguous():
+        raise ValueError(f"row_start: contiguous int32 [{n_seq + 1}] expected")
+    tshape, tstride = table.shape, table.stride()
+    if table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != n_seq or (tshape[1] > 1 and tstride[1] != 1):
         raise ValueError(f"table: int32 [{n_seq}, pages] with contiguous rows expected")
-    dev = rows.device
-    for t in (k_pages, v_pages, table, row_start, pos0, k_scale, v_scale):
-        if t is not None and _dev(t).device != dev:
-            raise ValueError("all tensors of a call must be on one device")
-    cache = capi.KvPages(ptr(k_pages), ptr(v_pages), ptr(k_scale), ptr(v_scale), n_pages, stride[0] if n_pages > 1 else 0, type_, size, n_kv, hd)
-    batch = capi.PageBatch(ptr(row_start), ptr(pos0), ptr(table), rows.shape[0], n_seq, table.shape[1], max(table.stride(0), table.shape[1]))
+    if dev < 0 or not dev == k_pages.get_device() == v_pages.get_device() == table.get_device() == row_start.get_device() == pos0.get_device():
+        raise ValueError("expected CUDA tensors of one device: this library has no CPU path")
+    cache = capi.KvPages(k_pages.data_ptr(), v_pages.data_ptr(), *scales, n_pages, stride[0] if n_pages > 1 else 0, type_, size, n_kv, hd)
+    batch = capi.PageBatch(row_start.data_ptr(), pos0.data_ptr(), table.data_ptr(), rows.shape[0], n_seq, tshape[1], max(tstride[0], tshape[1]))
     return cache, batch
 
 
 def _page_rows(x, heads, hd):
     """x as [rows, heads, hd] whose rows the kernels can read where they are, else a copy"""
-    if x.dtype not in _ROW_TYPES:
+    type_, shape, s = _ROW_TYPES.get(x.dtype), x.shape, x.stride()
+    if type_ is None:
         raise ValueError(f"rows of {x.dtype}: float32, float16 or bfloat16 expected")
-    if x.dim() != 3 or x.shape[1] != heads or x.shape[2] != hd:
-        raise ValueError(f"rows of shape {tuple(x.shape)}: [rows, {heads}, {hd}] expected")
-    s, es = x.stride(), x.element_size()
-    ok = s[2] == 1 and (s[1] == hd or heads == 1) and s[0] >= heads * hd and s[0] * es % 16 == 0 and x.data_ptr() % 16 == 0
+    if len(shape) != 3 or shape[1] != heads or shape[2] != hd:
+        raise ValueError(f"rows of shape {tuple(shape)}: [rows, {heads}, {hd}] expected")
+    per = 4 if type_ == TYPE_F32 else 8  # elements of 16 bytes
+    ok = s[2] == 1 and (s[1] == hd or heads == 1) and s[0] >= heads * hd and s[0] % per == 0 and x.data_ptr() % 16 == 0
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
+@contextlib.contextmanager
 def _on(dev):
-    """the caller's device and stream stay what they are: the kernels run on the current stream of the tensors' device"""
-    return torch.cuda.device(dev) if torch.cuda.current_device() != dev.index else contextlib.nullcontext()
+    """the caller's device stays what it is: the kernels run on the current stream of the tensors' device"""
+    with torch.cuda.device(dev):
+        yield
+
+
+@functools.lru_cache(maxsize=256)
+def _pages_scratch(dev, hd, n_kv, n_head, max_rows):
+    """a function of sizes alone (and of the device's multiprocessors)"""
+    with torch.cuda.device(dev):
+        return lib().b200_attention_pages_scratch_bytes(C.byref(capi.KvPages(None, None, None, None, 0, 0, 0, 0, n_kv, hd)), n_head, max_rows)
 
 
 def kv_pages_append(k, v, k_pages, v_pages, table, row_start, pos0, theta, neox, k_scale=None, v_scale=None):
     """k, v: [rows, n_kv, hd] (f32, f16, bf16; rows may be views of a wider projection) of a ragged batch: sequence s owns rows row_start[s] ..
     row_start[s + 1] - 1, at positions pos0[s] on; k is rotated there (theta 0: not), both go into the pages that table[s] names"""
-    _dev(k), _dev(v)
-    n_kv, hd = k_pages.shape[1], k_pages.shape[3]
+    _, n_kv, _, hd = k_pages.shape
     k, v = _page_rows(k, n_kv, hd), _page_rows(v, n_kv, hd)
-    if v.dtype != k.dtype or v.shape != k.shape or v.device != k.device:
+    if v.dtype is not k.dtype or v.shape != k.shape or v.get_device() != k.get_device():
         raise ValueError("k and v must be alike")
     cache, batch = _pages_call(k, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale)
-    with _on(k.device):
-        check(lib().b200_kv_pages_append(C.byref(cache), C.byref(batch), _ROW_TYPES[k.dtype], ptr(k), k.stride(0), ptr(v), v.stride(0), theta, int(neox),
-                                         cur_stream()))
+    dev = k.get_device()
+    with contextlib.nullcontext() if dev == torch.cuda.current_device() else _on(dev):
+        check(lib().b200_kv_pages_append(cache, batch, _ROW_TYPES[k.dtype], k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), theta, neox,
+                                         capi.device_stream(dev)))
 
 
 def attention_pages(q, k_pages, v_pages, table, row_start, pos0, max_rows, theta, neox, window=0, scale=0.0, k_scale=None, v_scale=None, out=None):
     """q: [rows, n_head, hd] of the same batch, not yet rotated (theta 0: as they are used) -> [rows, n_head, hd] of q's type; a row sees the positions
     of its sequence up to its own, the last `window` of them if that is not 0.  max_rows: most rows of a sequence.  Rows that no sequence owns are
     not written."""
-    _dev(q)
-    hd = k_pages.shape[3]
-    q = _page_rows(q, q.shape[1] if q.dim() == 3 else 0, hd)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device or _page_rows(out, q.shape[1], hd) is not out:
-        raise ValueError("out must be like q, with 16-byte aligned rows")
+    _, n_kv, _, hd = k_pages.shape
+    n_head = q.shape[1] if q.dim() == 3 else 0
+    q = _page_rows(q, n_head, hd)
     cache, batch = _pages_call(q, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale)
-    with _on(q.device):
-        need = lib().b200_attention_pages_scratch_bytes(C.byref(cache), q.shape[1], max_rows)
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
-        check(lib().b200_attention_pages(C.byref(cache), C.byref(batch), _ROW_TYPES[q.dtype], ptr(q), q.stride(0), q.shape[1], max_rows, theta, int(neox),
-                                         window, scale, ptr(out), out.stride(0), ptr(scratch), need, cur_stream()))
+    dev = q.get_device()
+    if out is None:
+        out = q.new_empty(q.shape)
+    elif out.dtype is not q.dtype or out.shape != q.shape or out.get_device() != dev or _page_rows(out, n_head, hd) is not out:
+        raise ValueError("out must be like q, with 16-byte aligned rows")
+    need = _pages_scratch(dev, hd, n_kv, n_head, max_rows)
+    scratch = table.new_empty(need // 4 + 1)
+    with contextlib.nullcontext() if dev == torch.cuda.current_device() else _on(dev):
+        check(lib().b200_attention_pages(cache, batch, _ROW_TYPES[q.dtype], q.data_ptr(), q.stride(0), n_head, max_rows, theta, neox, window, scale,
+                                         out.data_ptr(), out.stride(0), scratch.data_ptr(), need, capi.device_stream(dev)))
     return out
