@@ -307,8 +307,8 @@ B200_API b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b200
                                           const void *k, int64_t k_stride, const void *v, int64_t v_stride, float theta,
                                           int32_t neox, void *stream);
 /* Causal attention of the batch's rows over their sequences' pages: head h of a row at position p sees positions
- * p - window + 1 .. p (window 0: from 0 on) that are there, of KV head h / (n_head / n_kv); a row that sees none is 0.
- * q, out: [rows][n_head][head_dim] of type f32, f16 or bf16, q_stride and out_stride elements between rows, 16-byte aligned;
+ * p - window + 1 .. p (window 0: from 0 on; at most 2^30) that are there, of KV head h / (n_head / n_kv); a row that sees none is 0.
+ * q, out (which must not overlap): [rows][n_head][head_dim] of type f32, f16 or bf16, q_stride and out_stride elements between rows, 16-byte aligned;
  * the queries are rotated on the way in (theta 0: as they come).  scale 0: 1 / sqrt(head_dim).  max_rows: the most rows of a
  * sequence as far as the caller knows; it picks the kernels, any value is right.  f32: queries and probabilities enter
  * the products in two f16 parts, results are good to 32 bits; f16, bf16: probabilities in one f16 part.

@@ -611,7 +611,7 @@ b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_bat
     KQ_REQUIRE(theta >= 0.f && isfinite(theta), "attention_pages: rotation base %g", theta);
     KQ_REQUIRE(scale >= 0.f && isfinite(scale), "attention_pages: scale %g", scale);
     KQ_REQUIRE(a.b.rows * (int64_t)n_head <= 0x3fffffff, "attention_pages: %d rows of %d heads", a.b.rows, n_head);
-    KQ_REQUIRE(window >= 0 && max_rows >= 0, "attention_pages: window %d, rows %d", window, max_rows);
+    KQ_REQUIRE(window >= 0 && window <= (1 << 30) && max_rows >= 0, "attention_pages: window %d, rows %d", window, max_rows);
     if (a.b.rows == 0 || a.b.n_seq == 0) return B200_OK;
     const int hd = cache->head_dim;
     KQ_TRY(kq_rows_check("attention_pages", "queries", q, type, q_stride, (int64_t)n_head * hd));

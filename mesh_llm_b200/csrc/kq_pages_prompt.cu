@@ -141,10 +141,24 @@ struct Walk {
         kh = (int)kq_div(run.off, run.per_head);
         uo = run.off - kh * run.per_head;
         tiles = kq_tiles<R>(a, sq.t);
-        for (tile = 0;; tile++) {
-            const int n = kq_units<BK>(kq_tile_keys<R>(a, sq, tile)) + kq_setup<R>;
-            if (uo < n || tile + 1 >= tiles) break;
-            uo -= n;
+        // the tile that the run begins in: a lane counts one of 32
+        const int lane = threadIdx.x & 31;
+        for (tile = 0; tile < tiles; tile += 32) {
+            const int mine = tile + lane < tiles ? kq_units<BK>(kq_tile_keys<R>(a, sq, tile + lane)) + kq_setup<R> : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, (long long)upto > uo);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                uo -= __shfl_sync(0xffffffffu, upto - mine, l);
+                tile += l;
+                break;
+            }
+            uo -= __shfl_sync(0xffffffffu, upto, 31);
         }
     }
     // the next piece; false: no more
@@ -181,7 +195,6 @@ template <bool F8> __device__ __forceinline__ void less_registers() {
     if (F8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 }
-__device__ __noinline__ float2 turn_out_of_line(uint64_t f, int pos) { return kq_turn(f, pos); }
 // codes of 8 dimensions as f16 numbers times the block's scale
 __device__ __forceinline__ uint4 decode8(uint32_t lo, uint32_t hi, __half2 s) {
     auto two = [&](uint32_t v) {
@@ -434,8 +447,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         while (w.next(a)) {
             const int row0 = w.tile * R + 128 * half; // of this half, within the sequence and KV head
             // ---- queries: a warp's 32 rows are copied to where they will stand as f16 parts (which is as large), all in flight together, and then turned
-            // in place, four at a time; rows of one token share its angles.  (Eight rows at a time with the angles in line is 60 KB of code, and
-            // fetching it took four times as long as running it.)
+            // in place, four at a time.  The angles of the warp's tokens (rows of one share them) are worked out meanwhile, in a loop of their own: in line with the rows they
+            // are 60 KB of code, and fetching it took four times as long as running it; out of line the calls spill what the rows hold.
             constexpr int P = HD / 64, NB = 4, CH = HD * (int)sizeof(T) / 16; // 16-byte chunks of a row
             const bool split = a.turns.on && a.turns.neox;
             const int wrow = (warp & 3) * 32, tok0 = (row0 + wrow) / a.G, h0 = row0 + wrow - tok0 * a.G;
@@ -455,12 +468,21 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(raw_at(wrow + r, c))), "l"(src), "r"(there ? 16 : 0) : "memory");
                 }
             }
-            asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            float4 cs[33]; // of the lane's pairs, by token; in local memory
+            const int toks = min((h0 + 31) / a.G + 1, w.sq.t - tok0);
+#pragma unroll 2
+            for (int i = 0; i < toks; i++) {
+                float2 x = make_float2(1.f, 0.f), y = x;
+                if (a.turns.on) {
+                    x = kq_turn(sh.turns[P * lane], w.sq.pos(tok0 + i));
+                    y = P == 2 ? kq_turn(sh.turns[P * lane + P - 1], w.sq.pos(tok0 + i)) : x;
+                }
+                cs[i] = make_float4(x.x, x.y, y.x, y.y);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
-            float2 cs[P];
-#pragma unroll
-            for (int u = 0; u < P; u++) cs[u] = make_float2(1.f, 0.f);
-            int tok = tok0, h = h0, tok_cs = -1;
+            int tok = 0, h = h0; // token of the next row, counted from tok0, and its head
             // the lane's pairs are P lane + u: dimensions (pair, pair + HD / 2) or (2 pair, 2 pair + 1)
 #pragma unroll 1
             for (int rb = 0; rb < 32; rb += NB) {
@@ -476,13 +498,9 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 };
 #pragma unroll
                 for (int k = 0; k < NB; k++) {
-                    if (a.turns.on && tok != tok_cs && tok < w.sq.t) {
-                        tok_cs = tok;
-#pragma unroll
-                        for (int u = 0; u < P; u++) cs[u] = turn_out_of_line(sh.turns[P * lane + u], w.sq.pos(tok_cs));
-                    }
-#pragma unroll
-                    for (int u = 0; u < P; u++) c[k][u] = cs[u];
+                    const float4 v = tok < toks ? cs[tok] : make_float4(1.f, 0.f, 1.f, 0.f);
+                    c[k][0] = make_float2(v.x, v.y);
+                    c[k][P - 1] = P == 2 ? make_float2(v.z, v.w) : c[k][0];
                     if (++h == a.G) h = 0, tok++;
                 }
 #pragma unroll

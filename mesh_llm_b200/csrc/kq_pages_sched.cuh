@@ -57,12 +57,13 @@ template <int R, int U> __device__ __forceinline__ long long kq_head_units(const
     }
     if (q.p0 < 0) return (long long)tiles * (1 + kq_setup<R>);
     long long n = 0;
-    const int64_t cap = (int64_t)a.c.table_len * a.c.page;
+    const int cap = a.c.table_len * a.c.page, room = cap - q.p0; // new tokens that have a place; below 2^31 by the checks
     const int dq = R / a.G, dr = R % a.G;
     int last = (R - 1) / a.G, rem = (R - 1) % a.G;
 #pragma unroll 4
     for (int i = 0; i < tiles; i++) {
-        n += (uint32_t)(max(min((int64_t)q.p0 + min(last, q.t - 1) + 1, cap), (int64_t)1) + U - 1) / (uint32_t)U + kq_setup<R>;
+        const int seen = min(min(last, q.t - 1) + 1, room);
+        n += ((uint32_t)max(q.p0 + seen, 1) + U - 1u) / U + kq_setup<R>;
         last += dq;
         rem += dr;
         if (rem >= a.G) {
