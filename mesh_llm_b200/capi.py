@@ -280,11 +280,3 @@ def cur_stream():
     import torch
 
     return torch.cuda.current_stream().cuda_stream
-
-
-def device_stream(dev):
-    """the current stream of device `dev` as an integer, without an object around it (3 us where a call takes 10)"""
-    import torch
-
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return get(dev) if get else torch.cuda.current_stream(dev).cuda_stream

@@ -6,7 +6,6 @@ weights [N, K-bytes] uint8, activations [M, K] float32.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import functools
 
@@ -266,6 +265,9 @@ def moe_route(logits, k, mask=None):
 
 
 _PAGE_TYPES = {torch.float16: TYPE_F16, torch.float8_e4m3fn: TYPE_F8_E4M3}
+# without an object around it the current stream costs 0.1 us to ask for, with one 3 of the 10 that a call takes
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _ROW_TYPES = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
 
 
@@ -325,13 +327,6 @@ def _page_rows(x, heads, hd):
     return x if ok else x.clone(memory_format=torch.contiguous_format)
 
 
-@contextlib.contextmanager
-def _on(dev):
-    """the caller's device stays what it is: the kernels run on the current stream of the tensors' device"""
-    with torch.cuda.device(dev):
-        yield
-
-
 @functools.lru_cache(maxsize=256)
 def _pages_scratch(dev, hd, n_kv, n_head, max_rows):
     """a function of sizes alone (and of the device's multiprocessors)"""
@@ -348,9 +343,10 @@ def kv_pages_append(k, v, k_pages, v_pages, table, row_start, pos0, theta, neox,
         raise ValueError("k and v must be alike")
     cache, batch = _pages_call(k, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale)
     dev = k.get_device()
-    with contextlib.nullcontext() if dev == torch.cuda.current_device() else _on(dev):
-        check(lib().b200_kv_pages_append(cache, batch, _ROW_TYPES[k.dtype], k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), theta, neox,
-                                         capi.device_stream(dev)))
+    if dev != _device_now():  # the kernels run on the current stream of the tensors' device; the caller's device stays what it is
+        with torch.cuda.device(dev):
+            return kv_pages_append(k, v, k_pages, v_pages, table, row_start, pos0, theta, neox, k_scale, v_scale)
+    check(lib().b200_kv_pages_append(cache, batch, _ROW_TYPES[k.dtype], k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), theta, neox, _stream_of(dev)))
 
 
 def attention_pages(q, k_pages, v_pages, table, row_start, pos0, max_rows, theta, neox, window=0, scale=0.0, k_scale=None, v_scale=None, out=None):
@@ -362,13 +358,15 @@ def attention_pages(q, k_pages, v_pages, table, row_start, pos0, max_rows, theta
     q = _page_rows(q, n_head, hd)
     cache, batch = _pages_call(q, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale)
     dev = q.get_device()
+    if dev != _device_now():
+        with torch.cuda.device(dev):
+            return attention_pages(q, k_pages, v_pages, table, row_start, pos0, max_rows, theta, neox, window, scale, k_scale, v_scale, out)
     if out is None:
         out = q.new_empty(q.shape)
     elif out.dtype is not q.dtype or out.shape != q.shape or out.get_device() != dev or _page_rows(out, n_head, hd) is not out:
         raise ValueError("out must be like q, with 16-byte aligned rows")
     need = _pages_scratch(dev, hd, n_kv, n_head, max_rows)
-    scratch = table.new_empty(need // 4 + 1)
-    with contextlib.nullcontext() if dev == torch.cuda.current_device() else _on(dev):
-        check(lib().b200_attention_pages(cache, batch, _ROW_TYPES[q.dtype], q.data_ptr(), q.stride(0), n_head, max_rows, theta, neox, window, scale,
-                                         out.data_ptr(), out.stride(0), scratch.data_ptr(), need, capi.device_stream(dev)))
+    scratch = table.new_empty(need // 4)
+    check(lib().b200_attention_pages(cache, batch, _ROW_TYPES[q.dtype], q.data_ptr(), q.stride(0), n_head, max_rows, theta, neox, window, scale,
+                                     out.data_ptr(), out.stride(0), scratch.data_ptr(), need, _stream_of(dev)))
     return out
