@@ -448,9 +448,9 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         while (w.next(a)) {
             const int row0 = w.tile * R + 128 * half; // of this half, within the sequence and KV head
             // ---- queries: a warp's 32 rows are copied to where they will stand as f16 parts (which is as large), all in flight together, and then turned
-            // in place, four at a time.  The angles of the warp's tokens (rows of one share them) are worked out meanwhile, in a loop of their own: in line with the rows they
+            // in place, eight at a time.  The angles of the warp's tokens (rows of one share them) are worked out meanwhile, in a loop of their own: in line with the rows they
             // are 60 KB of code, and fetching it took four times as long as running it; out of line the calls spill what the rows hold.
-            constexpr int P = HD / 64, NB = 4, CH = HD * (int)sizeof(T) / 16; // 16-byte chunks of a row
+            constexpr int P = HD / 64, NB = 8, CH = HD * (int)sizeof(T) / 16; // 16-byte chunks of a row
             const bool split = a.turns.on && a.turns.neox;
             const int wrow = (warp & 3) * 32, tok0 = (row0 + wrow) / a.G, h0 = row0 + wrow - tok0 * a.G;
             auto raw_at = [&](int r, int c) { // chunk c of row r of this half
@@ -459,14 +459,15 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             };
             {
                 constexpr int STEP = 32 / CH; // rows of one copy of the warp
-                int ctok = tok0, ch = h0 + lane / CH;
-                const int c = lane % CH;
+                const int c = lane % CH, left = (w.sq.t - tok0) * a.G - h0; // rows of the sequence and KV head from the warp's first on
+                int ch = h0 + lane / CH;
+                const T *src = (const T *)a.q + (int64_t)(w.sq.row0 + tok0) * a.q_stride + (int64_t)(w.kh * a.G + ch) * HD + c * (16 / (int)sizeof(T));
+                const int64_t turn = a.q_stride - (int64_t)a.G * HD; // from behind a token's heads to the next token's
 #pragma unroll 4
-                for (int r = lane / CH; r < 32; r += STEP, ch += STEP) {
-                    while (ch >= a.G) ch -= a.G, ctok++;
-                    const bool there = ctok < w.sq.t;
-                    const T *src = (const T *)a.q + (there ? (int64_t)(w.sq.row0 + ctok) * a.q_stride + (int64_t)(w.kh * a.G + ch) * HD + c * (16 / (int)sizeof(T)) : 0);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(raw_at(wrow + r, c))), "l"(src), "r"(there ? 16 : 0) : "memory");
+                for (int r = lane / CH; r < 32; r += STEP, ch += STEP, src += STEP * HD) {
+                    while (ch >= a.G) ch -= a.G, src += turn;
+                    const bool there = r < left;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(raw_at(wrow + r, c))), "l"(there ? src : (const T *)a.q), "r"(there ? 16 : 0) : "memory");
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
