@@ -251,7 +251,8 @@ template <int HD, bool F8, typename T, bool SPLIT> b200_status launch(const KqPa
         KQ_CUDA(cudaFuncSetAttribute(pages_append_kernel<HD, F8, T, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::SMEM));
         if (dev >= 0 && dev < 64) attr[dev] = true;
     }
-    // few rows per sequence: a CTA per row, those of a sequence's later rows in a block have nothing to do; many: a CTA per 16 rows
+    // few rows per sequence: a CTA per row, those of a sequence's later rows in a block have nothing to do; many: a CTA per 16 rows, which takes their
+    // blocks one after another (256 sequences of a row 12.5 us with the first, 40 with the second; 4000 rows of one sequence 35 and 16)
     const int group = b.rows < 16 * (int64_t)b.n_seq ? 1 : KQ_PAGE_BLOCK;
     const dim3 grid((unsigned)kq_div_up(b.rows, group), (unsigned)kq_div_up(c.n_kv, HEADS));
     kq_launch(pages_append_kernel<HD, F8, T, SPLIT>, grid, WARPS * 32, M::SMEM, st, c, b, r, group, turns);

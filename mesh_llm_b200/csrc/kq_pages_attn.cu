@@ -573,7 +573,8 @@ template <int HD> b200_status launch(const KqAttnArgs &a, bool f8, int ht, cudaS
     return combine(a, HD, 8 * ht, ctas, st);
 }
 
-// Sequences of up to FEW rows of a KV head go to the kernel above, longer ones to the one for prompts, where the caller says there are any
+// Sequences of up to FEW rows of a KV head go to the kernel above, longer ones to the one for prompts, where the caller says there are any.
+// Measured, 16 sequences at 3000 of 4 KV heads, f16 pages, f32, here and there: 16 rows 34 and 88 us, 48 rows 65 and 90, 96 rows 110 and 92.
 constexpr int64_t FEW = 64;
 bool prompts(int64_t G, int64_t max_rows) { return G * max_rows > FEW; }
 

@@ -266,8 +266,9 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         const uint64_t dq = tc_desc(smem_u32(sm), 16, 1024), dk = tc_desc(ring, 16, 1024), dv = tc_desc(ring, HALF, 1024);
         uint32_t pieces = 0, units = 0, ks = 0, kph = 0; // slot of the next tile of the ring and the parity of its round
         bool ok = true;
+        bool both = true; // the second tile has rows
         auto scores = [&](int half, uint32_t slot) {
-            if (!lead || !ok) return;
+            if (!lead || !ok || (half && !both)) return;
             const uint64_t b = dk + slot * (L::TILE / 16);
 #pragma unroll
             for (int p = 0; p < QS; p++)
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             for (int x = 0; x < 2; x++) {
                 ok = wait_all(sh.p_ready[half][x], units & 1, 3) && ok;
                 after_sync();
-                if (lead && ok) {
+                if (lead && ok && (!half || both)) {
 #pragma unroll
                     for (int p = 0; p < PS; p++)
 #pragma unroll
@@ -296,6 +297,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             if (++slot == NS) slot = 0, ph ^= 1;
         };
         while (w.next(a)) {
+            both = w.sq.t * a.G - w.tile * R > 128;
             ok = wait_all(sh.q_ready, pieces & 1, 1) && ok;
             ok = wait_all(sh.full[ks], kph, 2) && ok;
             after_sync();
@@ -445,8 +447,34 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
         const int half = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), ts = tl + COL_S + 128 * half, to = tl + COL_O + 128 * half;
         uint32_t pieces = 0, units = 0;
+        // f16 values that no row sees may hold anything: they must not meet a probability of 0.  The first half's threads have a position of the tile each
+        auto hide_values = [&](int key0, int seen) {
+            if (F8 || half || (key0 + BK <= w.keys.y && key0 >= seen)) return;
+            const uint32_t v = 2 * units + 1;
+            wait(sh.full[v % NS], (v / NS) & 1, 11);
+            if (key0 + row >= w.keys.y || key0 + row < seen) {
+                uint8_t *d = sm + L::RING + (v % NS) * L::TILE + row * 128;
+#pragma unroll
+                for (int j = 0; j < HD / 8; j++) *reinterpret_cast<uint4 *>(d + (j >> 3) * HALF + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async();
+        };
         while (w.next(a)) {
             const int row0 = w.tile * R + 128 * half; // of this half, within the sequence and KV head
+            const int seen = a.window > 0 ? max(0, w.sq.pos(w.tile * R / a.G) - a.window + 1) : 0; // before this no row sees anything
+            if (row0 + (warp & 3) * 32 >= w.sq.t * a.G) { // none of the warp's rows is one: what the products make of its places is not looked at
+                arrive(smem_u32(&sh.q_ready));
+                for (int i = 0; i < w.take; i++, units++) {
+                    wait(sh.s_ready[half], units & 1, 10);
+                    hide_values(w.keys.x + (w.ub + i) * BK, seen);
+                    arrive(smem_u32(&sh.p_ready[half][0]));
+                    arrive(smem_u32(&sh.p_ready[half][1]));
+                }
+                wait(sh.o_done, pieces & 1, 12);
+                pieces++;
+                w.done();
+                continue;
+            }
             // ---- queries: a warp's 32 rows are copied to where they will stand as f16 parts (which is as large), all in flight together, and then turned
             // in place, eight at a time.  The angles of the warp's tokens (rows of one share them) are worked out meanwhile, in a loop of their own: in line with the rows they
             // are 60 KB of code, and fetching it took four times as long as running it; out of line the calls spill what the rows hold.
@@ -572,7 +600,6 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             const bool my_row_ok = (row0 + row) / a.G < w.sq.t;
             const int my_tok = min((row0 + row) / a.G, w.sq.t - 1), lim = w.sq.p0 < 0 ? -1 : w.sq.pos(my_tok); // last position this row sees
             const int lim_lo = w.sq.pos(min(row0 / a.G, w.sq.t - 1)), lim_hi = w.sq.pos(min((row0 + 127) / a.G, w.sq.t - 1)); // of the half's rows
-            const int seen = a.window > 0 ? max(0, w.sq.pos(w.tile * R / a.G) - a.window + 1) : 0;
             auto look_up = [&](int i) { // is the lane's block (of 32 from unit i on) there
                 const int key = w.keys.x + (w.ub + i) * BK + KQ_PAGE_BLOCK * lane;
                 return key < w.keys.y ? kq_page_of(a.c, w.s, key) : -1;
@@ -666,17 +693,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     }
                 }
                 const float sub = m == -INFINITY ? 0.f : m - 6.f; // probabilities up to 2^14: small ones keep their bits in f16
-                if (!F8 && half == 0 && (key0 + BK > w.keys.y || key0 < seen)) {
-                    // a value that no row sees may hold anything: it must not meet a probability of 0
-                    const uint32_t v = 2 * units + 1;
-                    wait(sh.full[v % NS], (v / NS) & 1, 11);
-                    if (key0 + row >= w.keys.y || key0 + row < seen) {
-                        uint8_t *d = sm + L::RING + (v % NS) * L::TILE + row * 128;
-#pragma unroll
-                        for (int j = 0; j < HD / 8; j++) *reinterpret_cast<uint4 *>(d + (j >> 3) * HALF + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_async();
-                }
+                hide_values(key0, seen);
                 uint64_t sums[2] = {0, 0};
                 uint32_t lo_even[PS == 2 ? 16 : 1];
                 const uint64_t crow2 = pack2(crow, crow), nsub2 = pack2(-sub, -sub);

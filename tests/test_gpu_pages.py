@@ -391,3 +391,15 @@ def test_offsets_past_32_bits():
     ops.kv_pages_append(x[:256], x[:256], z, z.clone(), torch.zeros((1, 1), dtype=torch.int32, device="cuda"), torch.tensor([0, 256], dtype=torch.int32, device="cuda"),
                         one.pos0 * 0, 1e6, 1)
     assert torch.equal(k2[n_pages - 1], z[0])
+
+
+@pytest.mark.parametrize("new", [33, 40, 65, 100, 129])
+def test_prompts_that_fill_part_of_a_tile(new):
+    """row tiles without a second half or with idle warps, over a last tile of keys whose other places hold NaN"""
+    for cache, hd in ((torch.float16, 128), (torch.float16, 64), (F8, 128)):
+        c, b = Cache(1, new + 150, 16, 1, hd, cache, seed=12), Batch([new], [70])
+        fill(c, [70], 130, 1e4, 1)
+        q = rows(39, new, 2, hd)
+        c.append(rows(40, new, 1, hd), rows(41, new, 1, hd), b, 1e4, 1)
+        for window in (0, 30):
+            close(c.attend(q, b, 1e4, 1, window=window), attention(c, q, b, 1e4, 1, window), torch.float32)
