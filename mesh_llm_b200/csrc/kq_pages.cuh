@@ -68,6 +68,8 @@ __device__ __forceinline__ uint32_t kq_e4m3x2_h2(uint16_t v) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
     return r;
 }
+// largest of a warp's values, none of them negative: their bits are in order
+__device__ __forceinline__ float kq_warp_top(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 // activations as f32
 template <typename T> __device__ __forceinline__ float2 kq_ld2(const T *p);
 template <> __device__ __forceinline__ float2 kq_ld2<float>(const float *p) { return *reinterpret_cast<const float2 *>(p); }
@@ -76,12 +78,6 @@ template <> __device__ __forceinline__ float2 kq_ld2<__nv_bfloat16>(const __nv_b
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(p));
 }
 template <typename T> __device__ __forceinline__ float kq_ld1(const T *p) { return (float)*p; }
-__device__ __forceinline__ float2 kq_ld2_type(uint32_t type, const void *p, int64_t at) {
-    return type == B200_TYPE_F32 ? kq_ld2((const float *)p + at) : type == B200_TYPE_F16 ? kq_ld2((const __half *)p + at) : kq_ld2((const __nv_bfloat16 *)p + at);
-}
-__device__ __forceinline__ float kq_ld1_type(uint32_t type, const void *p, int64_t at) {
-    return type == B200_TYPE_F32 ? ((const float *)p)[at] : type == B200_TYPE_F16 ? __half2float(((const __half *)p)[at]) : __bfloat162float(((const __nv_bfloat16 *)p)[at]);
-}
 __device__ __forceinline__ void kq_st2_type(uint32_t type, void *p, int64_t at, float a, float b) {
     if (type == B200_TYPE_F32) *reinterpret_cast<float2 *>((float *)p + at) = make_float2(a, b);
     else if (type == B200_TYPE_F16) *reinterpret_cast<__half2 *>((__half *)p + at) = __floats2half2_rn(a, b);

@@ -105,8 +105,8 @@ __device__ __forceinline__ void convert(const uint8_t *in, uint8_t *out, bool mi
 #pragma unroll
             for (int e = 0; e < 2 * P; e++) kmax = fmaxf(kmax, fabsf(k[e])), vmax = fmaxf(vmax, fabsf(v[e])); // a NaN does not count
         }
-        kmax = kq_warp_max(kmax);
-        vmax = kq_warp_max(vmax);
+        kmax = kq_warp_top(kmax);
+        vmax = kq_warp_top(vmax);
         if (lane == 0) top[0][warp] = kmax, top[1][warp] = vmax;
         __syncthreads(); // every warp has also read the old scales
 #pragma unroll

@@ -3,16 +3,19 @@
 // A CTA works on two tiles of 128 rows (row i of a sequence and KV head: token i / G, head i % G) that share every tile of 128 keys: while
 // the tensor cores multiply for one, the softmax warps of the other work.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with S (columns
 // 0 and 128) and O (256 and 384) in TMEM; a softmax thread owns a row: it writes its probabilities over scores that it has read, as f16, which
-// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 8 in base 2.  f32 queries go in as two f16 parts, and so do their probabilities; f16 queries, which the rotation makes longer than f16, go in as two.  As in the kernel for few rows a query row is
-// divided by the power of two of its largest element.
+// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 8 in base 2.  The first 64 keys'
+// part of the second product runs under the exponentials of the others.  f32 queries go in as two f16 parts, and so do their probabilities; f16
+// queries, which the rotation makes longer than f16, go in as two.  As in the kernel for few rows a query row is divided by the power of two of its
+// largest element.
 //
 // K and V tiles go through a ring in the order K0 V0 K1 V1 ...; f16 pages arrive by tiled TMA, 64 dimensions x 16 .. 128 positions of a page
 // to a box, with the 128-byte swizzle that both products read (V as an MN-major operand), pages that are not there as the zeros of an
 // out-of-range coordinate; e4m3 pages arrive as raw rows by bulk copies and four warps turn them into the f16 tile of what they stand for.
 //
-// Bound by the tensor pipe (4 x 512 clocks for 256 rows x 128 keys at head_dim 128) and as much by the exponentials (16 a clock: 2 x 1024).  Units are
-// shared out evenly over one CTA per SM (kq_pages_sched.cuh).  Every wait is bounded: on a time-out the kernel records
-// an error, lets its copies land, frees its TMEM and returns.
+// Bound, where items are long, by the tensor pipe (4 x 512 clocks for 256 rows x 128 keys at head_dim 128), the exponentials (16 a clock: 2 x 1024) and the
+// issue slots, all three near 2000 of the 3300 clocks that a unit takes; where they are short, by setting an item up (33 k clocks for a CTA's first, 27 k
+// for another).  4096 rows of 40 heads behind 12288 positions, bf16: 1.0 PFLOP/s.  Units are shared out evenly over one CTA per SM (kq_pages_sched.cuh).
+// Every wait is bounded: on a time-out the kernel records an error, lets its copies land, frees its TMEM and returns.
 #include "kq_pages_sched.cuh"
 #include "kq_tc.cuh"
 
@@ -120,7 +123,7 @@ template <int HD, bool F8, int QS> struct Layout {
 constexpr int MAX_SLOTS = 6;
 
 struct Shared {
-    uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], raw_full[4], raw_empty[4], s_ready[2], p_ready[2][2], o_done, q_ready;
+    uint64_t full[MAX_SLOTS], empty[MAX_SLOTS], raw_full[4], raw_empty[4], s_ready[2], p_ready[2][2], o_done, q_ready, drained;
     float crow[R];
     uint64_t turns[64]; // a lane's own entry is no broadcast: not from the constant bank
     uint32_t tmem;
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             init(sh.p_ready[i][1], 128); // and of the others
         }
         init(sh.o_done, 1);
+        init(sh.drained, 1);
         init(sh.q_ready, NSOFT);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.abort = 0;
@@ -341,6 +345,11 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             pieces++;
             w.done();
         }
+        if (!ok && lead) { // products in flight end before TMEM is freed
+            tc_commit(smem_u32(&sh.drained));
+            kq_mbar_wait(smem_u32(&sh.drained), 0, KQ_WAIT_LIMIT_NS);
+        }
+        __syncwarp();
     } else if (warp == 9) {
         less_registers<F8>();
         // ---------------------------------------------------------------- copies: a lane per box
@@ -479,6 +488,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             // in place, eight at a time.  The angles of the warp's tokens (rows of one share them) are worked out meanwhile, in a loop of their own: in line with the rows they
             // are 60 KB of code, and fetching it took four times as long as running it; out of line the calls spill what the rows hold.
             constexpr int P = HD / 64, NB = 8, CH = HD * (int)sizeof(T) / 16; // 16-byte chunks of a row
+            static_assert(NB == 8, "rows are swizzled by eights");
             const bool split = a.turns.on && a.turns.neox;
             const int wrow = (warp & 3) * 32, tok0 = (row0 + wrow) / a.G, h0 = row0 + wrow - tok0 * a.G;
             auto raw_at = [&](int r, int c) { // chunk c of row r of this half
@@ -515,17 +525,17 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             int tok = 0, h = h0; // token of the next row, counted from tok0, and its head
             // the lane's pairs are P lane + u: dimensions (pair, pair + HD / 2) or (2 pair, 2 pair + 1)
 #pragma unroll 1
-            for (int rb = 0; rb < 32; rb += NB) {
+            for (int rb = 0; rb < min(32, (w.sq.t - tok0) * a.G - h0); rb += NB) { // places behind the last row keep what they hold: nothing looks at them
                 float x[NB][P][2];
                 float2 c[NB][P];
-                auto pair_at = [&](int k, int d) { // elements d, d + 1
+                uint8_t *rows8 = sm + half * L::TILE + (wrow + rb) * 128; // eight rows, the place of each among eight is its swizzle
+                auto at8 = [&](int k, int d) { // element d of row k
                     constexpr int PER = 16 / (int)sizeof(T);
-                    return kq_ld2(reinterpret_cast<const T *>(raw_at(wrow + rb + k, d / PER)) + d % PER);
+                    const int c = d / PER, b = c >> 3;
+                    return reinterpret_cast<const T *>(rows8 + (HD == 128 ? (b >> 1) * (2 * L::TILE) + (b & 1) * HALF : b * (2 * L::TILE)) + k * 128 + (((c & 7) ^ k) << 4)) + d % PER;
                 };
-                auto one_at = [&](int k, int d) {
-                    constexpr int PER = 16 / (int)sizeof(T);
-                    return kq_ld1(reinterpret_cast<const T *>(raw_at(wrow + rb + k, d / PER)) + d % PER);
-                };
+                auto pair_at = [&](int k, int d) { return kq_ld2(at8(k, d)); };
+                auto one_at = [&](int k, int d) { return kq_ld1(at8(k, d)); };
 #pragma unroll
                 for (int k = 0; k < NB; k++) {
                     const float4 v = tok < toks ? cs[tok] : make_float4(1.f, 0.f, 1.f, 0.f);
@@ -563,9 +573,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     }
                 }
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-                    for (int k = 0; k < NB; k++) amax[k] = fmaxf(amax[k], __shfl_xor_sync(0xffffffffu, amax[k], o));
+                for (int k = 0; k < NB; k++) amax[k] = kq_warp_top(amax[k]);
 #pragma unroll
                 for (int k = 0; k < NB; k++) {
                     const int r = (warp & 3) * 32 + rb + k;
@@ -575,7 +583,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     auto put = [&](int d, float v0, float v1, bool two) { // dimension d (and d + 1)
 #pragma unroll
                         for (int p = 0; p < QS; p++) {
-                            uint8_t *at = sm + (2 * p + half) * L::TILE + (d >> 6) * HALF + r * 128 + ((((d >> 3) & 7) ^ (r & 7)) << 4) + (d & 7) * 2;
+                            uint8_t *at = rows8 + p * (2 * L::TILE) + (d >> 6) * HALF + k * 128 + ((((d >> 3) & 7) ^ k) << 4) + (d & 7) * 2;
                             const uint32_t hi = h2(v0, v1), v = p ? h2_low(v0, v1, hi) : hi;
                             if (two) *reinterpret_cast<uint32_t *>(at) = v;
                             else *reinterpret_cast<uint16_t *>(at) = (uint16_t)v;

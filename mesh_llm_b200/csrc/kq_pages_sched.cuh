@@ -3,9 +3,11 @@
 // An item is one tile of R rows (row i of a sequence and KV head: new token i / G, query head i % G) of one sequence and KV head; its keys
 // are cut into units of U positions.  All units of all items in order (sequence, head, tile, key) are cut into equal runs, one per CTA, so that
 // the longest sequence does not decide how long the launch takes.  What an item costs besides its keys (queries in, rows out) counts as kq_setup
-// units in front of its own; a CTA whose run ends among those leaves the item to the next.  A CTA's run is at most the end of one item (its partial result goes into slot
-// 2 cta), whole items (results go out), and the beginning of another (slot 2 cta + 1); meta[cta] describes the item that begins there and
-// goes on in other CTAs, and the combining kernel joins its slots in order.  Nothing depends on timing.
+// units in front of its own; a CTA whose run ends among those leaves the item to the next.
+//
+// A CTA's run is at most the end of one item (its partial result goes into slot 2 cta), whole items (results go out), and the beginning of another
+// (slot 2 cta + 1); meta[cta] describes the item that begins there and goes on in other CTAs, and a second kernel joins its slots in order.
+// Nothing depends on timing.
 #pragma once
 #include "kq_pages.cuh"
 
@@ -16,7 +18,7 @@ struct KqAttnArgs {
     void *out;
     int64_t q_stride, out_stride;
     uint32_t type;
-    int32_t n_head, G, window;
+    int32_t G, window;
     int64_t t_lo, t_hi; // sequences with t_lo <= rows x G <= t_hi are this kernel's
     float scale_log2;
     KqTurns turns;
