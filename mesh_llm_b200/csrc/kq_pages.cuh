@@ -63,10 +63,9 @@ __device__ __forceinline__ uint16_t kq_e4m3x2(float lo, float hi) { // round to 
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-__device__ __forceinline__ uint32_t kq_e4m3x2_h2(uint16_t v) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
-    return r;
+// four codes as two pairs of f16 (halves of a register as they are: no shift to reach the upper two)
+__device__ __forceinline__ void kq_e4m3x4_h2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 // largest of a warp's values, none of them negative: their bits are in order
 __device__ __forceinline__ float kq_warp_top(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }

@@ -125,7 +125,8 @@ __device__ __forceinline__ void convert(const uint8_t *in, uint8_t *out, bool mi
                     for (int x = part * 32 + lane; x < off * HD / 4; x += 32 * WH) {
                         uint32_t *w = reinterpret_cast<uint32_t *>(n ? vp : kp) + x;
                         const uint32_t c = *w;
-                        const uint32_t h0 = kq_e4m3x2_h2((uint16_t)c), h1 = kq_e4m3x2_h2((uint16_t)(c >> 16));
+                        uint32_t h0, h1;
+                        kq_e4m3x4_h2(c, h0, h1);
                         const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h0)), b = __half22float2(*reinterpret_cast<const __half2 *>(&h1));
                         *w = (uint32_t)kq_e4m3x2(a.x * ratio, a.y * ratio) | ((uint32_t)kq_e4m3x2(b.x * ratio, b.y * ratio) << 16);
                     }

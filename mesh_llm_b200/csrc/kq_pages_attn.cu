@@ -28,8 +28,9 @@ constexpr int NT = 128, NW = NT / 32;
 constexpr int MAX_CTAS_PER_SM = 3;
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes to shared memory, zeros where `there` is false (nothing is read then)
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+// zeros where `there` is false (nothing is read then)
+__device__ __forceinline__ void copy16_if(uint32_t dst, const void *src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t dst, const void *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
@@ -165,12 +166,23 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                         have |= (p >= 0) << n;
                         constexpr int CH = ROW / 16, PER = 16 * CH / 32; // chunks of a row; copies of a lane
                         const uint32_t dst = ring_u + st * S::STEP;
+                        const uint8_t *src_k = a.c.k + off + lane * 16, *src_v = a.c.v + off + lane * 16; // a block is one run: copy j of a lane is 512 j on
+                        const int kg = key0 + 16 * n;
+                        if (p >= 0 && kg + 16 <= keys.y && kg >= first_seen) {
 #pragma unroll
-                        for (int j = 0; j < PER; j++) {
-                            const int x = j * 32 + lane, r = x / CH, c = x % CH, key = key0 + 16 * n + r;
-                            const bool there = p >= 0 && key < keys.y && key >= first_seen; // what no row sees may hold anything: it must not meet a probability of 0
-                            copy16(dst + place<ROW>(16 * n + r, c), a.c.k + off + r * ROW + c * 16, there);
-                            copy16(dst + KT * ROW + place<ROW>(16 * n + r, c), a.c.v + off + r * ROW + c * 16, there);
+                            for (int j = 0; j < PER; j++) {
+                                const int x = j * 32 + lane;
+                                copy16(dst + place<ROW>(16 * n + x / CH, x % CH), src_k + 512 * j);
+                                copy16(dst + KT * ROW + place<ROW>(16 * n + x / CH, x % CH), src_v + 512 * j);
+                            }
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < PER; j++) {
+                                const int x = j * 32 + lane, key = kg + x / CH;
+                                const bool there = p >= 0 && key < keys.y && key >= first_seen; // what no row sees may hold anything: it must not meet a probability of 0
+                                copy16_if(dst + place<ROW>(16 * n + x / CH, x % CH), src_k + 512 * j, there);
+                                copy16_if(dst + KT * ROW + place<ROW>(16 * n + x / CH, x % CH), src_v + 512 * j, there);
+                            }
                         }
                         if (F8 && p >= 0 && lane < 2)
                             copy4(smem_u32(&sc_s[warp][st][2 * lane + n]), (lane ? a.c.vs : a.c.ks) + ((int64_t)p * a.c.n_kv + kh) * bpp + ib);
@@ -262,8 +274,9 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
 #pragma unroll
                                 for (int x = 0; x < KS / KL; x++) {
                                     const int ks = j * (KS / KL) + x;
-                                    const uint32_t b0 = F8 ? kq_e4m3x2_h2((uint16_t)word(kr, x)) : word(kr, 2 * x);
-                                    const uint32_t b1 = F8 ? kq_e4m3x2_h2((uint16_t)(word(kr, x) >> 16)) : word(kr, 2 * x + 1);
+                                    uint32_t b0, b1;
+                                    if (F8) kq_e4m3x4_h2(word(kr, x), b0, b1);
+                                    else b0 = word(kr, 2 * x), b1 = word(kr, 2 * x + 1);
                                     mma(c, qh[ks], b0, b1);
                                     if (SPLIT && HT == 2) mma(c, ql[SPLIT && HT == 2 ? ks : 0], b0, b1);
                                 }
@@ -361,10 +374,8 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                                 const uint32_t pick = i & 1 ? 0x7362u : 0x5140u;
                                 const uint32_t x = __byte_perm(word(vr[n][0][0], i >> 1), word(vr[n][1][0], i >> 1), pick);
                                 const uint32_t y = __byte_perm(word(vr[n][2][0], i >> 1), word(vr[n][3][0], i >> 1), pick);
-                                va[0] = kq_e4m3x2_h2((uint16_t)x);
-                                va[1] = kq_e4m3x2_h2((uint16_t)(x >> 16));
-                                va[2] = kq_e4m3x2_h2((uint16_t)y);
-                                va[3] = kq_e4m3x2_h2((uint16_t)(y >> 16));
+                                kq_e4m3x4_h2(x, va[0], va[1]);
+                                kq_e4m3x4_h2(y, va[2], va[3]);
                             } else {
                                 const uint32_t w0 = word(vr[n][0][i >> 2], i & 3), w1 = word(vr[n][1][i >> 2], i & 3);
                                 const uint32_t w2 = word(vr[n][2][i >> 2], i & 3), w3 = word(vr[n][3][i >> 2], i & 3);

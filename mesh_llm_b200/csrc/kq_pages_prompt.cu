@@ -201,12 +201,15 @@ template <bool F8> __device__ __forceinline__ void less_registers() {
 }
 // codes of 8 dimensions as f16 numbers times the block's scale
 __device__ __forceinline__ uint4 decode8(uint32_t lo, uint32_t hi, __half2 s) {
-    auto two = [&](uint32_t v) {
-        const uint32_t h = kq_e4m3x2_h2((uint16_t)v);
+    uint4 v;
+    kq_e4m3x4_h2(lo, v.x, v.y);
+    kq_e4m3x4_h2(hi, v.z, v.w);
+    auto scaled = [&](uint32_t &h) {
         const __half2 r = __hmul2(*reinterpret_cast<const __half2 *>(&h), s);
-        return *reinterpret_cast<const uint32_t *>(&r);
+        h = *reinterpret_cast<const uint32_t *>(&r);
     };
-    return make_uint4(two(lo), two(lo >> 16), two(hi), two(hi >> 16));
+    scaled(v.x), scaled(v.y), scaled(v.z), scaled(v.w);
+    return v;
 }
 
 // T: the activations' type; f32 and f16 queries in two f16 parts, probabilities of f32 results in two
