@@ -302,7 +302,8 @@ typedef struct b200_page_batch {
  * v_stride elements apart, 16-byte aligned.  Rows of a block of e4m3 positions go in under the larger of its scale
  * (where it holds earlier positions, whose codes are rescaled) and what the largest new value asks for.  A value beyond the
  * page type's range becomes the largest one; a NaN in v becomes 0 there and NaN at its place in the token's k, so
- * that exactly the queries that see the token give NaN.  Two sequences of one call must not write the same page.  */
+ * that exactly the queries that see the token give NaN.  No block of 16 positions may be written twice in one call (two
+ * sequences, or two table entries, that name one page): which of them it then holds is not defined.              */
 B200_API b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type,
                                           const void *k, int64_t k_stride, const void *v, int64_t v_stride, float theta,
                                           int32_t neox, void *stream);

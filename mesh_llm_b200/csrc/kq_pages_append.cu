@@ -274,7 +274,7 @@ KqTurns kq_turns(float theta, int neox, int hd) {
     t.neox = neox != 0;
     const double ratio = t.on ? pow((double)theta, -2.0 / hd) : 0.0; // one power: 63 products are off by 10^-14
     double f = t.on ? 1.0 / 6.283185307179586476925 : 0.0;
-    for (int i = 0; i < 64; i++, f *= ratio) t.f[i] = i < hd / 2 ? (uint64_t)(f * 18446744073709551616.0) : 0;
+    for (int i = 0; i < 64; i++, f *= ratio) t.f[i] = i < hd / 2 ? (uint64_t)((f - floor(f)) * 18446744073709551616.0) : 0; // a base below 1 turns faster than once a position
     return t;
 }
 
@@ -292,7 +292,7 @@ b200_status kq_pages_check(const char *who, const b200_kv_pages *c, const b200_p
     KQ_REQUIRE(stride >= page && stride * es % 16 == 0 && stride <= ((int64_t)1 << 36), "%s: page stride %lld (at least a page of %lld elements, a multiple of 16 bytes)", who, (long long)stride,
                (long long)page);
     KQ_REQUIRE(b->n_seq >= 0 && b->rows >= 0 && b->rows <= 0x3fffffff, "%s: %d sequences, %lld rows", who, b->n_seq, (long long)b->rows);
-    KQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->pos0 && b->table), "%s: row starts, positions and page table required", who);
+    KQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->pos0 && (b->table || b->table_len == 0)), "%s: row starts, positions and page table required", who);
     KQ_REQUIRE(((((uintptr_t)b->row_start | (uintptr_t)b->pos0 | (uintptr_t)b->table)) & 3) == 0, "%s: row starts, positions and page table must be 4-byte aligned", who);
     KQ_REQUIRE(b->table_len >= 0 && b->table_stride >= b->table_len, "%s: page table of %d entries, %d apart", who, b->table_len, b->table_stride);
     KQ_REQUIRE((int64_t)b->table_len * c->page_size <= 0x7fffffff, "%s: %d pages of %d positions are more than 2^31 - 1 positions", who, b->table_len, c->page_size);

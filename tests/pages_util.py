@@ -10,7 +10,7 @@ def turned(x, pos, theta, neox):
     x = x.double()
     if theta == 0:
         return x
-    hd = x.shape[-1]
+    hd, theta = x.shape[-1], float(np.float32(theta))  # the base is an f32 number
     a = pos.double()[:, None] * theta ** (-torch.arange(hd // 2, dtype=torch.float64, device=x.device) * 2 / hd)
     c, s = a.cos()[:, None], a.sin()[:, None]
     u, w = (x[..., :hd // 2], x[..., hd // 2:]) if neox else (x[..., 0::2], x[..., 1::2])

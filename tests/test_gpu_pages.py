@@ -403,3 +403,96 @@ def test_prompts_that_fill_part_of_a_tile(new):
         c.append(rows(40, new, 1, hd), rows(41, new, 1, hd), b, 1e4, 1)
         for window in (0, 30):
             close(c.attend(q, b, 1e4, 1, window=window), attention(c, q, b, 1e4, 1, window), torch.float32)
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+def test_a_prompt_in_chunks_and_steps_is_the_prompt_at_once(cache):
+    """append and attention together as an engine uses them: chunks of any size, then single tokens, against one call and against 64 bits"""
+    n, n_kv, n_head, hd, theta = 400, 2, 10, 128, 1e6
+    q, k, v = rows(50, n, n_head, hd), rows(51, n, n_kv, hd), rows(52, n, n_kv, hd)
+    one, many = (Cache(1, n, 48, n_kv, hd, cache, seed=13) for _ in "ab")
+    b = Batch([n], [0])
+    one.append(k, v, b, theta, 1)
+    whole = one.attend(q, b, theta, 1)
+    parts, at = [], 0
+    for t in (1, 130, 5, 16, 200, 17) + (1,) * 31:
+        step = Batch([t], [at])
+        many.append(k[at:at + t], v[at:at + t], step, theta, 1)
+        parts.append(many.attend(q[at:at + t], step, theta, 1))
+        at += t
+    assert at == n
+    close(whole, attention(one, q, b, theta, 1), torch.float32)
+    close(parts[-1], attention(many, q, b, theta, 1)[n - 1:], torch.float32)
+    if cache == torch.float16:  # e4m3: a block's earlier rows were quantised under the scale it had then
+        close(torch.cat(parts), attention(one, q, b, theta, 1), torch.float32)
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+def test_scratch_of_any_content_and_two_graphs_on_it(cache):
+    import ctypes as C
+
+    from mesh_llm_b200 import capi, ops
+
+    new, past = [300, 1, 40], [100, 900, 0]
+    c, b = Cache(3, 1000, 32, 2, 128, cache, seed=14), Batch(new, past)
+    fill(c, past, 140, 1e4, 1)
+    q = rows(53, b.rows, 16, 128)
+    c.append(rows(54, b.rows, 2, 128), rows(55, b.rows, 2, 128), b, 1e4, 1)
+    want = c.attend(q, b, 1e4, 1)
+    pages, batch = ops._pages_call(q, c.k, c.v, c.table, b.start, b.pos0, c.ks, c.vs)
+    need = capi.lib().b200_attention_pages_scratch_bytes(pages, 16, b.most)
+    scratch = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")  # NaN everywhere
+    out = [torch.zeros_like(q) for _ in "ab"]
+
+    def call(o):
+        capi.check(capi.lib().b200_attention_pages(pages, batch, 0, q.data_ptr(), q.stride(0), 16, b.most, 1e4, 1, 0, 0.0, o.data_ptr(), o.stride(0),
+                                                   scratch.data_ptr(), need, capi.cur_stream()))
+
+    call(out[0])
+    assert torch.equal(out[0], want)
+    graphs = [torch.cuda.CUDAGraph() for _ in "ab"]
+    for g, o in zip(graphs, out):
+        with torch.cuda.graph(g):
+            call(o)
+    for o in out:
+        o.zero_()
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    assert torch.equal(out[0], want) and torch.equal(out[1], want)
+
+
+@pytest.mark.parametrize("theta", [0.01, 0.7, 1.0, 1e9])
+def test_rotation_bases(theta):
+    c, b = Cache(1, 4000, 16, 1, 64, torch.float16), Batch([3], [3990])
+    k = rows(56, 3, 1, 64)
+    c.append(k, k, b, theta, 0)
+    want = turned(k, torch.arange(3990, 3993, device="cuda"), theta, 0)
+    # fast turns: a frequency of f turns a position is a 64-bit fraction of one, rounded from 53 bits
+    assert ((c.rows(0, 3993)[0][3990:] - want).abs() <= want.abs() * 2.0 ** -11 + k.abs().max().double() * 2.0 ** -21).all()
+
+
+def test_calls_on_two_streams_at_once():
+    c, b = Cache(4, 2000, 16, 2, 128, torch.float16, seed=15), Batch([1] * 4, [1999, 100, 700, 5])
+    fill(c, [2000, 101, 701, 6], 150, 1e4, 1)
+    q = rows(57, 4, 8, 128)
+    want = c.attend(q, b, 1e4, 1)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(30):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(c.attend(q, b, 1e4, 1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+def test_tables_of_no_pages():
+    c = Cache(2, 32, 16, 1, 64, torch.float16)
+    c.table = torch.empty((2, 0), dtype=torch.int32, device="cuda")
+    b = Batch([1, 100], [5, 0])
+    before = c.k.clone()
+    c.append(rows(58, 101, 1, 64), rows(59, 101, 1, 64), b, 1e4, 1)
+    assert torch.equal(c.k.view(torch.int16), before.view(torch.int16))
+    assert (c.attend(rows(60, 101, 4, 64), b, 1e4, 1) == 0).all()
