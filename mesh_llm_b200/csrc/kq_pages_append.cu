@@ -1,6 +1,6 @@
 // New keys and values into the pages of their sequences, the keys rotated on the way (b200_kv_pages_append).
 //
-// One CTA takes the new rows that fall into one aligned block of 16 positions of one sequence and 4 heads: 16-byte asynchronous copies
+// One CTA takes the new rows that fall into one aligned block of 16 positions of one sequence and 4 or 8 heads: 16-byte asynchronous copies
 // bring them into shared memory while the CTA works out their cosines and sines, a lane turns and rounds the same pair of dimensions of every row of a
 // head, and the rows go out from shared memory again as whole runs of their page (from the lanes, where a pair is (i, i + hd / 2), they went out
 // a byte at a time: 11516 rows of 8 heads, bf16 into e4m3, 66 us against 38 with neighbouring pairs).  An e4m3 block is one CTA's own, so its scale (the smallest power of two that brings the largest of the new values to at
@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int WARPS = 8, HEADS = 4, WH = WARPS / HEADS; // WH warps of a head take every WH-th row
+constexpr int WH = 2; // warps of a head: each takes every second row
 
 struct Rows {
     const void *k, *v;
@@ -46,18 +46,19 @@ __device__ __forceinline__ float clamped(float x, float m) { // NaN stays
     return x < -m ? -m : x;
 }
 
-template <int HD, bool F8, typename T> struct Room { // shared memory: rows as they come, [keys, values][row][head][HD], and as they are stored, [keys, values][head][row][ROW]
-    static constexpr int ROW = HD * (F8 ? 1 : 2);
+template <int HD, bool F8, typename T, int H> struct Room { // shared memory: rows as they come, [keys, values][row][head][HD], and as they are stored, [keys, values][head][row][ROW]
+    static constexpr int HEADS = H, WARPS = WH * H, ROW = HD * (F8 ? 1 : 2);
     static constexpr int IN = KQ_PAGE_BLOCK * HEADS * HD * (int)sizeof(T), OUT = HEADS * KQ_PAGE_BLOCK * ROW, SMEM = 2 * (IN + OUT);
 };
 
 // The new rows of one block from `in` to `out`.  A lane has P = HD / 64 neighbouring pairs of dimensions of a row, P lane ...: (pair, pair + HD / 2) if SPLIT,
 // else (2 pair, 2 pair + 1).  For an e4m3 block the rows are turned twice, for the largest value and again for the codes: kept in registers they would
 // halve the CTAs on an SM.
-template <int HD, bool F8, typename T, bool SPLIT>
+template <int HD, bool F8, typename T, bool SPLIT, int H>
 __device__ __forceinline__ void convert(const uint8_t *in, uint8_t *out, bool mine, uint8_t *kp, uint8_t *vp, float *ks, float *vs, float old_k, float old_v, int off, int cnt,
-                                        const float2 (*cs)[HD / 2], float (*top)[WARPS], bool on) {
-    using M = Room<HD, F8, T>;
+                                        const float2 (*cs)[HD / 2], float (*top)[WH * H], bool on) {
+    using M = Room<HD, F8, T, H>;
+    constexpr int HEADS = H;
     constexpr int P = HD / 64;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % WH, head = warp / WH;
     // elements of a row as they stand: 2 P of them from d0 on, or P from d0 and P from d0 + HD / 2
@@ -170,10 +171,11 @@ __device__ __forceinline__ void convert(const uint8_t *in, uint8_t *out, bool mi
 }
 
 // grid (groups of `group` rows, heads in parts).  A CTA takes the blocks whose first new row is in its group.
-template <int HD, bool F8, typename T, bool SPLIT>
-__global__ void __launch_bounds__(WARPS * 32, 4) pages_append_kernel(const __grid_constant__ KqPages c, const __grid_constant__ KqBatch b, const __grid_constant__ Rows r, int group,
+template <int HD, bool F8, typename T, bool SPLIT, int H>
+__global__ void __launch_bounds__(WH * H * 32, 16 / H) pages_append_kernel(const __grid_constant__ KqPages c, const __grid_constant__ KqBatch b, const __grid_constant__ Rows r, int group,
                                                                      const __grid_constant__ KqTurns turns) {
-    using M = Room<HD, F8, T>;
+    using M = Room<HD, F8, T, H>;
+    constexpr int HEADS = M::HEADS, WARPS = M::WARPS;
     extern __shared__ __align__(16) uint8_t room[];
     __shared__ float2 cs[KQ_PAGE_BLOCK][HD / 2];
     __shared__ uint64_t turns_s[HD / 2]; // a lane's own entry is no broadcast: not from the constant bank
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) pages_append_kernel(const __gri
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncthreads();
             uint8_t *out = room + 2 * M::IN;
-            convert<HD, F8, T, SPLIT>(room, out, mine, c.k + code, c.v + code, c.ks + sc, c.vs + sc, old_k, old_v, off, cnt, cs, top, turns.on);
+            convert<HD, F8, T, SPLIT, H>(room, out, mine, c.k + code, c.v + code, c.ks + sc, c.vs + sc, old_k, old_v, off, cnt, cs, top, turns.on);
             __syncthreads();
             // a head's new rows are one run of its page
             constexpr int PER = KQ_PAGE_BLOCK * M::ROW / 16;
@@ -243,27 +245,35 @@ __global__ void __launch_bounds__(WARPS * 32, 4) pages_append_kernel(const __gri
     }
 }
 
-template <int HD, bool F8, typename T, bool SPLIT> b200_status launch(const KqPages &c, const KqBatch &b, const Rows &r, const KqTurns &turns, cudaStream_t st) {
-    using M = Room<HD, F8, T>;
+template <int HD, bool F8, typename T, bool SPLIT, int H> b200_status launch(const KqPages &c, const KqBatch &b, const Rows &r, const KqTurns &turns, cudaStream_t st) {
+    using M = Room<HD, F8, T, H>;
     static bool attr[64];
     int dev = 0;
     KQ_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !attr[dev]) {
-        KQ_CUDA(cudaFuncSetAttribute(pages_append_kernel<HD, F8, T, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::SMEM));
+        KQ_CUDA(cudaFuncSetAttribute(pages_append_kernel<HD, F8, T, SPLIT, H>, cudaFuncAttributeMaxDynamicSharedMemorySize, M::SMEM));
         if (dev >= 0 && dev < 64) attr[dev] = true;
     }
     // few rows per sequence: a CTA per row, those of a sequence's later rows in a block have nothing to do; many: a CTA per 16 rows, which takes their
     // blocks one after another (256 sequences of a row 12.5 us with the first, 40 with the second; 4000 rows of one sequence 35 and 16)
     const int group = b.rows < 16 * (int64_t)b.n_seq ? 1 : KQ_PAGE_BLOCK;
-    const dim3 grid((unsigned)kq_div_up(b.rows, group), (unsigned)kq_div_up(c.n_kv, HEADS));
-    kq_launch(pages_append_kernel<HD, F8, T, SPLIT>, grid, WARPS * 32, M::SMEM, st, c, b, r, group, turns);
+    const dim3 grid((unsigned)kq_div_up(b.rows, group), (unsigned)kq_div_up(c.n_kv, H));
+    kq_launch(pages_append_kernel<HD, F8, T, SPLIT, H>, grid, M::WARPS * 32, M::SMEM, st, c, b, r, group, turns);
     KQ_COUNT_LAUNCH();
     KQ_LAUNCH_CHECK();
     return B200_OK;
 }
-template <int HD, bool F8, typename T> auto pick(bool split) { return split ? launch<HD, F8, T, true> : launch<HD, F8, T, false>; }
-template <int HD, bool F8> auto pick(uint32_t type, bool split) {
-    return type == B200_TYPE_F32 ? pick<HD, F8, float>(split) : type == B200_TYPE_F16 ? pick<HD, F8, __half>(split) : pick<HD, F8, __nv_bfloat16>(split);
+// heads of a CTA: 4, or 8 where rows and codes of 8 take less than half an SM (16-bit rows into e4m3: 11516 rows of 8 heads 30 us instead of 32;
+// into f16 36 instead of 30); they share their angles
+template <int HD, bool F8, typename T> b200_status launch(const KqPages &c, const KqBatch &b, const Rows &r, const KqTurns &turns, cudaStream_t st) {
+    const bool split = turns.on && turns.neox;
+    if constexpr (F8 && sizeof(T) == 2)
+        if (c.n_kv > 4) return split ? launch<HD, F8, T, true, 8>(c, b, r, turns, st) : launch<HD, F8, T, false, 8>(c, b, r, turns, st);
+    return split ? launch<HD, F8, T, true, 4>(c, b, r, turns, st) : launch<HD, F8, T, false, 4>(c, b, r, turns, st);
+}
+template <int HD, bool F8> b200_status launch(uint32_t type, const KqPages &c, const KqBatch &b, const Rows &r, const KqTurns &turns, cudaStream_t st) {
+    if (type == B200_TYPE_F32) return launch<HD, F8, float>(c, b, r, turns, st);
+    return type == B200_TYPE_F16 ? launch<HD, F8, __half>(c, b, r, turns, st) : launch<HD, F8, __nv_bfloat16>(c, b, r, turns, st);
 }
 
 } // namespace
@@ -320,7 +330,7 @@ extern "C" b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b2
     KQ_TRY(kq_rows_check("kv_pages_append", "values", v, type, v_stride, width));
     const Rows r{k, v, k_stride, v_stride};
     const KqTurns turns = kq_turns(theta, neox, cache->head_dim);
-    const bool f8 = cache->type == B200_TYPE_F8_E4M3, split = turns.on && turns.neox;
-    auto *go = cache->head_dim == 128 ? (f8 ? pick<128, true>(type, split) : pick<128, false>(type, split)) : (f8 ? pick<64, true>(type, split) : pick<64, false>(type, split));
-    return go(c, b, r, turns, (cudaStream_t)stream);
+    const bool f8 = cache->type == B200_TYPE_F8_E4M3;
+    if (cache->head_dim == 128) return f8 ? launch<128, true>(type, c, b, r, turns, (cudaStream_t)stream) : launch<128, false>(type, c, b, r, turns, (cudaStream_t)stream);
+    return f8 ? launch<64, true>(type, c, b, r, turns, (cudaStream_t)stream) : launch<64, false>(type, c, b, r, turns, (cudaStream_t)stream);
 }

@@ -22,7 +22,7 @@ struct KqAttnArgs {
     int64_t t_lo, t_hi; // sequences with t_lo <= rows x G <= t_hi are this kernel's
     float scale_log2;
     KqTurns turns;
-    float *part; // [2 CTAs][R][HD + 2]: unnormalised rows, then (maximum, sum) of each
+    float *part; // [2 CTAs][R (HD + 2)]: a slot is R unnormalised rows, then (maximum, sum) of each
     int4 *meta;  // [CTAs][2]: pieces (0: none), KV head, tile, -; first row and number of rows of the sequence, -, -
 };
 
