@@ -12,8 +12,8 @@
 // rows; f32 and f16 rows go in as two f16 parts (rotation makes an f16 query longer than f16), and so do their probabilities; the tensor cores
 // cut their sums off instead of rounding them, so those of one step (16 or 32 keys) are added to the row in 32-bit registers.
 //
-// Bound by HBM: a position costs 2 hd codes per KV head and is read once.  f16 pages, 200 sequences of 60 to 6000 positions: 5.9 TB/s, 0.95 of a copy's
-// rate; e4m3 pages, half the bytes for as much arithmetic: 4.3 TB/s, where the instruction streams around the conversions count as much.  The units of
+// Bound by HBM: a position costs 2 hd codes per KV head and is read once.  f16 pages, 200 sequences of 60 to 6000 positions: 6.2 TB/s, 0.95 of a copy's
+// rate; e4m3 pages, half the bytes for as much arithmetic: 4.4 TB/s, where the instruction streams around the conversions count as much.  The units of
 // all items are shared out evenly (kq_pages_sched.cuh), the four warps of a CTA take neighbouring positions and join their rows through shared memory at an item's end.
 #include "kq_pages_sched.cuh"
 
@@ -475,6 +475,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
 
 // CTA b: the item of up to 16 rows that begins in CTA b of the attention kernel and goes on in the next pieces - 1 of them.  A row's pieces are
 // shared out over 512 / 32 / R warps, whose lanes are the dimensions; eight pieces' loads are in flight together.
+// A chain of latencies: 7 us of the 55 of one sequence at 131000 (eight items of some 50 pieces).
 template <int HD, int R> __global__ void __launch_bounds__(512) pages_combine_kernel(const __grid_constant__ KqAttnArgs a) {
     constexpr int W = 16 / R, N = HD / 64; // warps of a row, pairs of dimensions of a lane
     __shared__ float2 o_s[16][HD / 2];

@@ -827,6 +827,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 }
 
 // joins the pieces of a split item: a warp for two rows, lanes the dimensions, four pieces' loads together; grid (CTAs of the attention kernel, R / 16)
+// 7 us where every item is split, most of it the launch and one chain of loads
 template <int HD> __global__ void __launch_bounds__(256) pages_join_kernel(const __grid_constant__ KqAttnArgs a) {
     KQ_PDL_ENTER();
     const int4 meta = a.meta[2 * blockIdx.x], seq = a.meta[2 * blockIdx.x + 1];
