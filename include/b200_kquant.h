@@ -281,7 +281,8 @@ B200_API b200_status b200_attention_kv(const float *q, const void *k_cache, cons
  * of two from 2^-15 to 2^7, so code times scale is an f16 number.  head_dim 64 or 128, page_size a multiple of 16.
  * A batch: row r of its `rows` rows belongs to the sequence s with row_start[s] <= r < row_start[s + 1] (ascending,
  * n_seq + 1 entries; rows no sequence owns are left alone) and stands at position pos0[s] + r - row_start[s];
- * table[s][i] is the page of positions i page_size .. of sequence s, table_len entries that are table_stride apart.
+ * table[s][i] is the page of positions i page_size .. of sequence s, table_len entries that are table_stride apart (together
+ * at most 2^31 - 4096 positions).
  * row_start, pos0 and table are device memory, read by the kernels: a captured graph follows what they hold at its replay.
  * A table entry outside 0 .. n_pages - 1, a position past the table and every position of a sequence with
  * pos0 < 0 are not there: neither stored nor seen.                                              */

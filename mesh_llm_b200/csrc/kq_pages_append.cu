@@ -306,7 +306,8 @@ b200_status kq_pages_check(const char *who, const b200_kv_pages *c, const b200_p
     KQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->pos0 && (b->table || b->table_len == 0)), "%s: row starts, positions and page table required", who);
     KQ_REQUIRE(((((uintptr_t)b->row_start | (uintptr_t)b->pos0 | (uintptr_t)b->table)) & 3) == 0, "%s: row starts, positions and page table must be 4-byte aligned", who);
     KQ_REQUIRE(b->table_len >= 0 && b->table_stride >= b->table_len, "%s: page table of %d entries, %d apart", who, b->table_len, b->table_stride);
-    KQ_REQUIRE((int64_t)b->table_len * c->page_size <= 0x7fffffff, "%s: %d pages of %d positions are more than 2^31 - 1 positions", who, b->table_len, c->page_size);
+    // the attention kernels' steps run up to 4095 positions past the last one
+    KQ_REQUIRE((int64_t)b->table_len * c->page_size <= 0x7ffff000, "%s: %d pages of %d positions are more than 2^31 - 4096 positions", who, b->table_len, c->page_size);
     *out = KqPages{(uint8_t *)c->k, (uint8_t *)c->v, c->k_scale, c->v_scale, b->table, c->n_pages, stride * es, b->table_len, b->table_stride, c->page_size, c->n_kv};
     *batch = KqBatch{b->row_start, b->pos0, (int32_t)b->rows, b->n_seq};
     return B200_OK;

@@ -43,7 +43,7 @@ template <int R> __device__ __forceinline__ int2 kq_tile_keys(const KqAttnArgs &
     const int first = tile * R / a.G, last = min(q.t - 1, (tile * R + R - 1) / a.G); // rows x heads stay below 2^30
     const int64_t cap = (int64_t)a.c.table_len * a.c.page;
     const int hi = q.p0 < 0 ? 0 : (int)min((int64_t)q.p0 + last + 1, cap);
-    const int lo = a.window > 0 ? (int)max((int64_t)0, (int64_t)q.p0 + first - a.window + 1) & ~(A - 1) : 0;
+    const int lo = a.window > 0 ? (int)min(max((int64_t)0, (int64_t)q.p0 + first - a.window + 1), cap) & ~(A - 1) : 0;
     return make_int2(min(lo, hi & ~(A - 1)), hi);
 }
 // Units that setting an item up counts as.  200 decode sequences of 60 to 6000 positions: 188 us without any, 114 with two.  Prompts of 512 rows at

@@ -367,6 +367,28 @@ def test_far_positions():
     close(y[1], w, torch.float32)
 
 
+@pytest.mark.parametrize("heads", [(2, 2), (1, 5)])
+@pytest.mark.parametrize("dtype", [torch.float16, F8])
+@pytest.mark.parametrize("window", [1, 1000, 1 << 30])
+def test_positions_past_32_bits(window, dtype, heads):
+    """a sequence whose rows pass position 2^31 - 1, far behind its table: it stores nothing, sees nothing, and disturbs no other"""
+    n_kv, n_head = heads
+    c = Cache(3, 100, 16, n_kv, 64, dtype)
+    fill(c, [90, 90, 90], 60, 0.0, 1)
+    b = Batch([4, 300, 30], [86, 2 ** 31 - 9, 2 ** 31 - 1])
+    held = [x.clone().view(torch.uint8) for x in (c.k, c.v)]
+    ordinary = Batch([4, 0, 0], [86, 0, 0])
+    x = rows(61, b.rows, n_kv, 64)
+    c.append(x, x, Batch([0, 300, 30], b.past), 0.0, 1)
+    assert all(torch.equal(was, now.view(torch.uint8)) for was, now in zip(held, (c.k, c.v)))
+    q = rows(62, b.rows, n_head, 64)
+    want = attention(c, q, ordinary, 0.0, 1, window)
+    for most in (1, 300):  # either kernel
+        y = c.attend(q, b, 0.0, 1, window=window, max_rows=most)
+        assert (y[4:] == 0).all()
+        close(y[:4], want[:4], torch.float32)
+
+
 def test_offsets_past_32_bits():
     """the last page of a pool of more than 2^31 elements"""
     from mesh_llm_b200 import ops

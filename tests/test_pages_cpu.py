@@ -36,7 +36,7 @@ BAD_CACHE = [dict(type=0), dict(type=8), dict(head_dim=96), dict(head_dim=256), 
              dict(n_kv=0), dict(n_pages=0), dict(n_pages=1 << 40), dict(k=None), dict(v=P + 8), dict(page_stride=100), dict(page_stride=2 * 16 * 128 + 4),
              dict(type=capi.TYPE_F8_E4M3), dict(type=capi.TYPE_F8_E4M3, k_scale=P, v_scale=P + 2)]
 BAD_BATCH = [dict(rows=-1), dict(rows=1 << 40), dict(n_seq=-1), dict(row_start=None), dict(pos0=None), dict(table=None), dict(pos0=P + 2), dict(table_len=-1),
-             dict(table_len=5), dict(table_len=1 << 28, table_stride=1 << 28)]
+             dict(table_len=5), dict(table_len=1 << 28, table_stride=1 << 28), dict(table_len=(1 << 27) - 255, table_stride=1 << 27)]
 
 
 @pytest.mark.parametrize("bad", BAD_CACHE, ids=str)
