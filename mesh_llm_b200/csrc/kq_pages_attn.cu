@@ -632,6 +632,10 @@ b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_bat
     KQ_TRY(kq_rows_check("attention_pages", "results", out, type, out_stride, (int64_t)n_head * hd));
     KQ_REQUIRE(scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= b200_attention_pages_scratch_bytes(cache, n_head, max_rows),
                "attention_pages: scratch of %zu bytes, 16-byte aligned, required", b200_attention_pages_scratch_bytes(cache, n_head, max_rows));
+    const int64_t es = type == B200_TYPE_F32 ? 4 : 2, width = (int64_t)n_head * hd * es, apart = (const uint8_t *)out - (const uint8_t *)q, row = q_stride * es;
+    const int64_t in_row = ((apart % row) + row) % row; // where results begin in a row of queries, if both are parts of rows as long
+    KQ_REQUIRE(apart >= (a.b.rows - 1) * row + width || -apart >= (a.b.rows - 1) * out_stride * es + width || (q_stride == out_stride && in_row >= width && in_row + width <= row),
+               "attention_pages: results over queries");
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;

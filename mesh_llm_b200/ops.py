@@ -290,8 +290,8 @@ def _pages_call(rows, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale
     if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride:
         raise ValueError("pages: two pools [n_pages, n_kv, page_size, hd] of one shape and layout expected")
     n_pages, n_kv, size, hd = shape
-    if n_pages and stride[1:] != (size * hd, hd, 1):
-        raise ValueError("pages: each page must be contiguous")
+    if n_pages and (stride[1:] != (size * hd, hd, 1) or n_pages > 1 and stride[0] < n_kv * size * hd):
+        raise ValueError("pages: each page must be contiguous and its own")
     dev = rows.get_device()
     if type_ == TYPE_F8_E4M3:
         for s in (k_scale, v_scale):
@@ -306,12 +306,12 @@ def _pages_call(rows, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale
     if row_start.dtype is not torch.int32 or row_start.shape != (n_seq + 1,) or not row_start.is_contiguous():
         raise ValueError(f"row_start: contiguous int32 [{n_seq + 1}] expected")
     tshape, tstride = table.shape, table.stride()
-    if table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != n_seq or (tshape[1] > 1 and tstride[1] != 1):
-        raise ValueError(f"table: int32 [{n_seq}, pages] with contiguous rows expected")
+    if table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != n_seq or (tshape[1] > 1 and tstride[1] != 1) or (n_seq > 1 and not tshape[1] <= tstride[0] < 1 << 31):
+        raise ValueError(f"table: int32 [{n_seq}, pages] with contiguous rows, one for each sequence, expected")
     if dev < 0 or not dev == k_pages.get_device() == v_pages.get_device() == table.get_device() == row_start.get_device() == pos0.get_device():
         raise ValueError("expected CUDA tensors of one device: this library has no CPU path")
     cache = capi.KvPages(k_pages.data_ptr(), v_pages.data_ptr(), *scales, n_pages, stride[0] if n_pages > 1 else 0, type_, size, n_kv, hd)
-    batch = capi.PageBatch(row_start.data_ptr(), pos0.data_ptr(), table.data_ptr(), rows.shape[0], n_seq, tshape[1], max(tstride[0], tshape[1]))
+    batch = capi.PageBatch(row_start.data_ptr(), pos0.data_ptr(), table.data_ptr(), rows.shape[0], n_seq, tshape[1], tstride[0] if n_seq > 1 else tshape[1])
     return cache, batch
 
 
@@ -356,6 +356,8 @@ def attention_pages(q, k_pages, v_pages, table, row_start, pos0, max_rows, theta
     _, n_kv, _, hd = k_pages.shape
     n_head = q.shape[1] if q.dim() == 3 else 0
     q = _page_rows(q, n_head, hd)
+    if not 0 <= window <= 1 << 30 or not 0 <= max_rows < 1 << 31:
+        raise ValueError(f"window {window} (0 to 2^30), max_rows {max_rows} (0 to 2^31 - 1)")
     cache, batch = _pages_call(q, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale)
     dev = q.get_device()
     if dev != _device_now():

@@ -389,6 +389,25 @@ def test_positions_past_32_bits(window, dtype, heads):
         close(y[:4], want[:4], torch.float32)
 
 
+def test_results_beside_queries():
+    """queries and results as parts of one buffer's rows; results over the queries are refused"""
+    c = Cache(2, 60, 16, 2, 64, torch.float16)
+    fill(c, [40, 50], 70, 1e4, 1)
+    b = Batch([20, 3], [40, 50])
+    x = rows(71, b.rows, 2, 64)
+    c.append(x, x, b, 1e4, 1)
+    both = rows(72, b.rows, 8, 64)
+    q, out = both[:, :4], both[:, 4:]
+    want = attention(c, q, b, 1e4, 1)
+    for most in (1, 20):
+        assert c.attend(q, b, 1e4, 1, max_rows=most, out=out) is out
+        close(out, want, torch.float32)
+    with pytest.raises(RuntimeError, match="over queries"):
+        c.attend(q, b, 1e4, 1, out=both[:, 2:6])
+    with pytest.raises(RuntimeError, match="over queries"):
+        c.attend(q, b, 1e4, 1, out=q)
+
+
 def test_offsets_past_32_bits():
     """the last page of a pool of more than 2^31 elements"""
     from mesh_llm_b200 import ops

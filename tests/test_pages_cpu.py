@@ -26,7 +26,7 @@ def append(c=None, b=None, type=0, k=P, ks=256, v=P, vs=256, theta=1e4):
     return capi.lib().b200_kv_pages_append(C.byref(c or cache()), C.byref(b or batch()), type, k, ks, v, vs, theta, 1, None)
 
 
-def attend(c=None, b=None, type=0, q=P, qs=1024, n_head=8, most=1, theta=1e4, window=0, scale=0.0, out=P, os=1024, scratch=P, nbytes=1 << 40):
+def attend(c=None, b=None, type=0, q=P, qs=1024, n_head=8, most=1, theta=1e4, window=0, scale=0.0, out=2 * P, os=1024, scratch=P, nbytes=1 << 40):
     build.build()
     return capi.lib().b200_attention_pages(C.byref(c or cache()), C.byref(b or batch()), type, q, qs, n_head, most, theta, 1, window, scale, out, os,
                                            scratch, nbytes, None)
@@ -55,11 +55,16 @@ def test_append_arguments_refused(bad):
     assert append(**bad) == -1
 
 
-@pytest.mark.parametrize("bad", [dict(type=8), dict(q=None), dict(out=P + 8), dict(qs=1023), dict(os=1026), dict(n_head=7), dict(n_head=0), dict(n_head=8192), dict(window=-1),
+@pytest.mark.parametrize("bad", [dict(type=8), dict(q=None), dict(out=2 * P + 8), dict(qs=1023), dict(os=1026), dict(n_head=7), dict(n_head=0), dict(n_head=8192), dict(window=-1),
                                  dict(scale=-1.0), dict(scale=float("inf")), dict(theta=-2.0), dict(most=-1), dict(scratch=None), dict(scratch=P + 8), dict(nbytes=16),
                                  dict(b=batch(rows=1 << 29))], ids=str)
 def test_attention_arguments_refused(bad):
     assert attend(**bad) == -1
+
+
+@pytest.mark.parametrize("out, stride", [(P, 1024), (P + 16, 1024), (P + 2 * 4096 + 4080, 1024), (P - 2 * 4096 - 4080, 1024), (P + 4096, 2048), (P - 4096, 2048)], ids=str)
+def test_results_over_queries_refused(out, stride):
+    assert attend(out=out, os=stride) == -1  # queries: 3 rows of 4096 bytes from P on
 
 
 def test_nothing_to_do_is_no_launch():
@@ -78,6 +83,24 @@ def test_python_refuses_cpu_tensors_and_shapes():
         ops.kv_pages_append(x, x, pages, pages, i[None, :1], i, i[:1], 1e4, 1)
     with pytest.raises(ValueError):
         ops.attention_pages(x, pages, pages, i[None, :1], i, i[:1], 1, 1e4, 1)
+
+
+def test_python_refuses_shared_pages_and_tables():
+    """pools and tables whose rows lie over one another (expanded views), before the device is looked at"""
+    from mesh_llm_b200 import ops
+
+    x = torch.zeros((3, 2, 128))
+    pages = torch.zeros((4, 2, 16, 128), dtype=torch.float16)
+    i = torch.zeros(3, dtype=torch.int32)
+    table = torch.zeros((2, 4), dtype=torch.int32)
+    with pytest.raises(ValueError, match="its own"):
+        ops.kv_pages_append(x, x, pages[:1].expand(4, -1, -1, -1), pages[:1].expand(4, -1, -1, -1), table, i, i[:2], 1e4, 1)
+    for t in (table[:1].expand(2, -1), table.as_strided((2, 4), (2, 1)), table.T[:2]):
+        with pytest.raises(ValueError, match="contiguous rows"):
+            ops.kv_pages_append(x, x, pages, pages, t, i, i[:2], 1e4, 1)
+    for window, most in ((-1, 1), ((1 << 30) + 1, 1), ((1 << 32) + 5, 1), (0, -1), (0, 1 << 32)):
+        with pytest.raises(ValueError, match="window"):
+            ops.attention_pages(x, pages, pages, table, i, i[:2], most, 1e4, 1, window=window)
 
 
 def test_descriptor_layout():
