@@ -59,7 +59,7 @@ __device__ __forceinline__ float ex2(float x) {
 template <int HD, bool F8, int HT> struct Shape {
     static constexpr int R = 8 * HT, ES = F8 ? 1 : 2, ROW = HD * ES, NG = F8 ? 2 : 1, KT = 16 * NG; // groups of 16 positions of a warp's step
     static constexpr int STEP = 2 * KT * ROW;                                                       // keys, then values
-        static constexpr int NST = STEP == 8192 ? (HT == 1 ? 2 : 3) : 4; // ring stages of a warp
+    static constexpr int NST = STEP == 8192 ? (HT == 1 ? 2 : 3) : 4; // ring stages of a warp
     static constexpr int CTAS = HT == 1 ? 3 : 2;                     // per SM (2 of 3 stages each: 64 sequences 79 us instead of 75, 200 in 8 bits 208 instead of 188)
     static constexpr int SMEM = NW * NST * STEP;
     static_assert(NST * STEP >= R * HD * 4, "a warp's rows fit into its ring");
