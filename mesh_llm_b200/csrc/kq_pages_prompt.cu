@@ -29,12 +29,10 @@ namespace {
 constexpr int R = 256, BK = 128, NSOFT = 256;
 constexpr uint64_t LIMIT = 5 * KQ_WAIT_LIMIT_NS;
 constexpr uint32_t COL_S = 0, COL_O = 256;
-// f32: the tensor cores cut their sums off instead of rounding them, each step of 16 keys and part by half a last bit on average, which made rows
-// of 1800 keys to a piece 4e-6 too small.  So the row's sum of probabilities is cut off in the same steps (what is lost cancels where it is
-// divided by), and every FLUSH units O and the sum are put aside and added up in 32 bits.  512 rows of 40 heads at 1536, relative error against
-// 64 bits (plain 32-bit sums: 8.6e-7): 16 units 1.7e-6, 6 units 1.1e-6, 4 units 8.9e-7.
+// f32: the tensor cores cut their sums off instead of rounding them: of a product what lies below 2^-25 of the sum that it joins, of a step's sum what lies
+// below its 24 bits.  So every FLUSH units O and the row's sum of probabilities are put aside and added up in 32 bits, and the sum is taken of the parts that
+// O is made of, in O's steps and cut off as O's are: what a step loses there cancels where it is divided by, and where it loses nothing, neither does the sum.
 constexpr int FLUSH = 6;
-constexpr float CUT_HALF_BIT = 4.3e-8f; // half a last bit relative to the value, over mantissas of 1 to 2 as they come: 2^-24 / (2 ln 2)
 
 __device__ int g_pages_error;
 
@@ -705,15 +703,17 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 }
                 const float sub = m == -INFINITY ? 0.f : m - 6.f; // probabilities up to 2^14: small ones keep their bits in f16
                 hide_values(key0, seen);
-                uint64_t sums[2] = {0, 0};
+                uint64_t sums[2] = {0, 0}; // f32: of the steps of a chunk; else of all keys, in two runs
                 uint32_t lo_even[PS == 2 ? 16 : 1];
                 const uint64_t crow2 = pack2(crow, crow), nsub2 = pack2(-sub, -sub);
                 // a chunk's probabilities go over scores that have been read: those of keys 0 .. 63 to columns 0 .. 31 (second parts 32 .. 63) ...
 #pragma unroll
                 for (int h64 = 0; h64 < 2; h64++) {
                     uint32_t hi[16], lo[PS == 2 ? 16 : 1];
+                    float rest_sums[4]; // of the second parts, by step
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
+                        uint64_t rests[2] = {0, 0};
                         const int c = 2 * h64 + e;
                         uint32_t(&x)[32] = s[c];
 #pragma unroll
@@ -722,11 +722,16 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                             // results of 16 bits: 3 of 8 exponentials on the FMA pipe, so that neither it nor the special-function unit decides alone
                             // (4096 rows behind 12288 positions: 1509, 1480, 1460, 1437 us for 0, 1, 2, 3 of 8)
                             v = PS == 1 && j % 8 < POLY ? exp2_poly(v) : exp2_sfu(v);
-                            sums[PS == 2 ? j >> 3 : j & 1] = add2(sums[PS == 2 ? j >> 3 : j & 1], v);
+                            if (PS == 1) sums[j & 1] = add2(sums[j & 1], v);
                             const float2 p = unpack2(v);
                             hi[j] = h2(p.x, p.y);
                             if (PS == 2) {
-                                const uint32_t rest = h2_low(p.x, p.y, hi[j]);
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
+                                const uint64_t f2 = pack2(f.x, f.y), r2 = fma2(f2, pack2(-1.f, -1.f), v);
+                                sums[j >> 3] = add2(sums[j >> 3], f2);
+                                rests[j >> 3] = add2(rests[j >> 3], r2);
+                                const float2 r = unpack2(r2);
+                                const uint32_t rest = h2(r.x, r.y);
                                 if (e == 0) lo_even[PS == 2 ? j : 0] = rest;
                                 else lo[PS == 2 ? j : 0] = rest;
                             }
@@ -737,6 +742,13 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                                 const float2 v = unpack2(sums[g]);
                                 l = __fadd_rz(l, v.x + v.y);
                                 sums[g] = 0;
+                                const float2 r = unpack2(rests[g]);
+                                rest_sums[2 * e + g] = r.x + r.y;
+                            }
+                            if (e) {
+#pragma unroll
+                                for (int g = 0; g < 4; g++)
+                                    if (fabsf(rest_sums[g]) >= l * 0x1p-25f) l = __fadd_rz(l, rest_sums[g]);
                             }
                         }
                         if (!*abort) {
@@ -751,8 +763,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     before_sync();
                     arrive(smem_u32(&sh.p_ready[half][h64]));
                 }
-                if (PS == 2) l = fmaf(l, -8.f * CUT_HALF_BIT, l); // the second parts' eight steps
-                else {
+                if (PS == 1) {
                     const float2 v = unpack2(add2(sums[0], sums[1]));
                     l += v.x + v.y;
                 }
