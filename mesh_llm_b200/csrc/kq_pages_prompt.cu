@@ -3,7 +3,7 @@
 // A CTA works on two tiles of 128 rows (row i of a sequence and KV head: token i / G, head i % G) that share every tile of 128 keys: while
 // the tensor cores multiply for one, the softmax warps of the other work.  S = Q K^T and O += P V are tcgen05.mma kind::f16 with S (columns
 // 0 and 128) and O (256 and 384) in TMEM; a softmax thread owns a row: it writes its probabilities over scores that it has read, as f16, which
-// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 8 in base 2.  The first 64 keys'
+// are the A operand of the second product, and rescales its row of O only when its maximum has grown by more than 4 in base 2.  The first 64 keys'
 // part of the second product runs under the exponentials of the others.  f32 queries go in as two f16 parts, and so do their probabilities; f16
 // queries, which the rotation makes longer than f16, go in as two.  As in the kernel for few rows a query row is divided by the power of two of its
 // largest element.
@@ -30,9 +30,16 @@ constexpr int R = 256, BK = 128, NSOFT = 256;
 constexpr uint64_t LIMIT = 5 * KQ_WAIT_LIMIT_NS;
 constexpr uint32_t COL_S = 0, COL_O = 256;
 // f32: the tensor cores cut their sums off instead of rounding them: of a product what lies below 2^-25 of the sum that it joins, of a step's sum what lies
-// below its 24 bits.  So every FLUSH units O and the row's sum of probabilities are put aside and added up in 32 bits, and the sum is taken of the parts that
-// O is made of, in O's steps and cut off as O's are: what a step loses there cancels where it is divided by, and where it loses nothing, neither does the sum.
+// below its 24 bits.  So O and the row's sum of probabilities are put aside and added up in 32 bits every FLUSH units, and as soon as a unit has added less than
+// 1 / DOMINATED of what is there: what a unit of 128 keys loses is in proportion to what it joins, 1.9e-6 of that on average.  The sum is taken of the
+// parts that O is made of, in O's steps and cut off as O's are: what a step loses there cancels where it is divided by, and where it loses nothing, neither
+// does the sum.  Relative error with positive values, 512 rows of 40 heads behind 3000 keys: 3.6e-6 where all weigh alike, at most 8.1e-6 where one outweighs
+// the others (every six units alone 2.0e-5); values of either sign: 1.1e-6.  Four units instead of six: 2.3e-6 for 5 % of the time.
 constexpr int FLUSH = 6;
+constexpr float DOMINATED = 12.f;
+// Probabilities are worked out under 2^(m - PEAK), m the row's maximum when it last moved, and m moves when it would grow by more than GROWTH: they
+// stay below 2^(PEAK + GROWTH), and f16's smallest step of 2^-24 is 2^-35 of the largest.  (6 and 8: 60000 keys of e^-14 beside one of 1, 1.06e-5 off instead of 3.5e-6.)
+constexpr float PEAK = 11.f, GROWTH = 4.f;
 
 __device__ int g_pages_error;
 
@@ -315,7 +322,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             }
             __syncwarp();
             for (int i = 0; i < w.take; i++) {
-                const bool more = i + 1 < w.take, first = PS == 2 ? i % FLUSH == 0 : i == 0;
+                const bool more = i + 1 < w.take, first = i == 0;
                 uint32_t vs = ks, vph = kph;
                 next(vs, vph);
                 ks = vs, kph = vph;
@@ -618,6 +625,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             const int slot = 2 * blockIdx.x + (w.ub == 0 ? 1 : 0); // of a piece that is not the whole item
             // sums put aside: four columns of all rows next to one another, so that a warp's lanes write one run
             float *aside = a.part + (int64_t)gridDim.x * 2 * R * (HD + 2) + (int64_t)blockIdx.x * R * HD + 4 * (128 * half + row);
+            int joined = 0;     // units in O since it was put aside
+            float last_l = 0.f; // what the last one added to l
             float m = -INFINITY, l = 0.f, l_sum = 0.f, m_sum = -INFINITY; // l_sum: of what was put aside; m_sum: the maximum that it goes by
             // the row's O so far: what the tensor cores have summed and what was put aside before; as 32 columns a time
             auto total = [&](int k, uint32_t *o) {
@@ -644,7 +653,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 const int key0 = w.keys.x + (w.ub + i) * BK;
                 wait(sh.s_ready[half], units & 1, 10);
                 after_sync(); // S was issued behind the products before: O is at rest
-                if (PS == 2 && i > 0 && i % FLUSH == 0) {
+                if (PS == 2 && __any_sync(0xffffffffu, joined == FLUSH || (last_l > 0.f && l > DOMINATED * last_l))) {
 #pragma unroll
                     for (int k = 0; k < HD / 32; k++) {
                         uint32_t o[32];
@@ -652,11 +661,17 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
                             *reinterpret_cast<uint4 *>(aside + (8 * k + j / 4) * (4 * R)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) o[j] = 0;
+                        if (!*abort) tmem_st32(to + 32 * k, o);
                     }
+                    tmem_st_wait();
                     l_sum = l + (m_sum != -INFINITY ? l_sum * ex2(m_sum - m) : 0.f);
                     l = 0.f;
                     m_sum = m;
+                    joined = 0;
                 }
+                joined++;
                 const bool masked = blocks != 0xff || key0 + BK - 1 > lim_lo || (a.window > 0 && key0 <= lim_hi - a.window);
                 const int last = lim - key0, first = a.window > 0 ? last - a.window + 1 : -0x40000000;
                 auto mask = [&](uint32_t *s, int c) {
@@ -684,7 +699,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1]));
                 const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * crow;
-                const bool grown = !(top <= m + 8.f) || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
+                const bool grown = !(top <= m + GROWTH) || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
                 if (__any_sync(0xffffffffu, grown)) {
                     const float mn = grown ? max3(m, top, top) : m, alpha = mn == m ? 1.f : ex2(m - mn);
                     m = mn;
@@ -701,9 +716,10 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         }
                     }
                 }
-                const float sub = m == -INFINITY ? 0.f : m - 6.f; // probabilities up to 2^14: small ones keep their bits in f16
+                const float sub = m == -INFINITY ? 0.f : m - PEAK;
                 hide_values(key0, seen);
                 uint64_t sums[2] = {0, 0}; // f32: of the steps of a chunk; else of all keys, in two runs
+                const float l_before = l;
                 uint32_t lo_even[PS == 2 ? 16 : 1];
                 const uint64_t crow2 = pack2(crow, crow), nsub2 = pack2(-sub, -sub);
                 // a chunk's probabilities go over scores that have been read: those of keys 0 .. 63 to columns 0 .. 31 (second parts 32 .. 63) ...
@@ -763,7 +779,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     before_sync();
                     arrive(smem_u32(&sh.p_ready[half][h64]));
                 }
-                if (PS == 1) {
+                if (PS == 2) last_l = l - l_before;
+                else {
                     const float2 v = unpack2(add2(sums[0], sums[1]));
                     l += v.x + v.y;
                 }

@@ -55,3 +55,40 @@ def test_sums_that_lose_nothing(weight, hd, cache):
     got, want = c.attend(q, b, 0.0, 0, scale=1.0).double(), attention(c, q, b, 0.0, 0, scale=1.0)
     off = ((got - want).abs() / want.abs()).max().item()
     assert off <= 10 * 2.0 ** -24, off
+
+
+def some_rows(scores, values, new, past, n_head):
+    """rows and what they are, from the definition in 64 bits: the queries are alike, so the heads of a KV head are too"""
+    at = sorted({0, 1, new // 2, new - 1})
+    out = []
+    for r in at:
+        n = past + r + 1
+        w = torch.softmax(scores[:n].double(), 0)
+        out.append(torch.einsum("nh,nhd->hd", w, values[:n].double()).repeat_interleave(n_head // values.shape[1], 0))
+    return at, torch.stack(out)
+
+
+def one_beside_many(below, ones, n, n_kv, hd):
+    """scores of the first key 0, of the others -below; values 1, or f16 numbers from 1 to 2"""
+    scores = torch.full((n, n_kv), -below, device="cuda")
+    scores[0] = 0
+    g = torch.Generator("cuda").manual_seed(2)
+    values = torch.ones((n, n_kv, hd), device="cuda")
+    if not ones:
+        values += torch.rand(values.shape, generator=g, device="cuda")
+    return scores, values.half().float()
+
+
+@pytest.mark.parametrize("below, ones, n_kv, new, past, bound", [(10.0, False, 8, 512, 3000, 1.2e-5), (14.0, True, 8, 512, 3000, 1.2e-5), (16.0, True, 8, 512, 3000, 1.2e-5),
+                                                                 (18.0, False, 8, 512, 3000, 1.2e-5), (14.0, False, 4, 1280, 60000, 1e-5)])
+def test_one_key_that_outweighs_many(below, ones, n_kv, new, past, bound):
+    """A large weight, then thousands of small ones whose products are cut off at 2^-25 of the sum.  O is put aside once a unit has added little, so two units of
+    128 keys can lose that much of each product: 7.6e-6; the cut-off results of their 32 steps, of which the divisor's take back half: 1e-6; the roundings of
+    the test above: 6e-7; the small weights among themselves, 4e-6 of their part, which is at most a half: 2e-6 (a twentieth behind 60000 keys: 2e-7); their f16 parts, 2^-25 each
+    where the large one is 2^11: 1e-6 behind 60000."""
+    scores, values = one_beside_many(below, ones, new + past, n_kv, 128)
+    c = filled(scores, values, 64, torch.float16)
+    at, want = some_rows(scores, values, new, past, 40)
+    got = c.attend(first_element(new, 40, 128), Batch([new], [past]), 0.0, 0, scale=1.0)[at].double()
+    off = ((got - want).abs() / want).max().item()
+    assert off <= bound, off
