@@ -313,7 +313,9 @@ B200_API b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b200
  * q, out (which must not overlap): [rows][n_head][head_dim] of type f32, f16 or bf16, q_stride and out_stride elements between rows, 16-byte aligned;
  * the queries are rotated on the way in (theta 0: as they come).  scale 0: 1 / sqrt(head_dim).  max_rows: the most rows of a
  * sequence as far as the caller knows; it picks the kernels, any value is right.  f32: queries and probabilities enter
- * the products in two f16 parts, results are good to 32 bits; f16, bf16: probabilities in one f16 part.
+ * the products in two f16 parts (in prompts what a product loses goes by the sum that it joins: up to 1e-5 of the row's largest
+ * partial sum, 1e-6 where values are of either sign); bf16: probabilities in one f16 part; f16: in two, in sequences of more than 64
+ * rows a KV head in one, whose roundings come to 1/4 half step of the result.
  * scratch: b200_attention_pages_scratch_bytes of device memory, 16-byte aligned, of any content; calls that share it must be
  * ordered on one stream.                                                                        */
 B200_API size_t b200_attention_pages_scratch_bytes(const b200_kv_pages *cache, int32_t n_head, int32_t max_rows);

@@ -222,6 +222,7 @@ template <int HD, bool F8, typename T>
 __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
     pages_prompt_kernel(const __grid_constant__ KqAttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box_rows) {
     constexpr int QS = std::is_same<T, __nv_bfloat16>::value ? 1 : 2, PS = std::is_same<T, float>::value ? 2 : 1;
+    constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     using L = Layout<HD, F8, QS>;
     constexpr int NS = L::NS, NR = L::NR > 0 ? L::NR : 1, NT = F8 ? 512 : 384;
     extern __shared__ __align__(1024) uint8_t sm_raw[];
@@ -735,15 +736,19 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
                             uint64_t v = fma2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), crow2, nsub2);
-                            // results of 16 bits: 3 of 8 exponentials on the FMA pipe, so that neither it nor the special-function unit decides alone
+                            // results of 8 bits: 3 of 8 exponentials on the FMA pipe, so that neither it nor the special-function unit decides alone
                             // (4096 rows behind 12288 positions: 1509, 1480, 1460, 1437 us for 0, 1, 2, 3 of 8)
-                            v = PS == 1 && j % 8 < POLY ? exp2_poly(v) : exp2_sfu(v);
-                            if (PS == 1) sums[j & 1] = add2(sums[j & 1], v);
+                            v = BF && j % 8 < POLY ? exp2_poly(v) : exp2_sfu(v);
+                            if (BF) sums[j & 1] = add2(sums[j & 1], v);
                             const float2 p = unpack2(v);
                             hi[j] = h2(p.x, p.y);
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
+                            const uint64_t f2 = pack2(f.x, f.y);
+                            // f16: the divisor is the sum of the weights as O has them, rounded, so that one weight's rounding is not the result's.  (Two parts
+                            // as in f32 take 2048 rows at 6144 from 385 to 484 us, for results 1.01 instead of 1.13 half steps off.)
+                            if (PS == 1 && !BF) sums[j & 1] = add2(sums[j & 1], f2);
                             if (PS == 2) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
-                                const uint64_t f2 = pack2(f.x, f.y), r2 = fma2(f2, pack2(-1.f, -1.f), v);
+                                const uint64_t r2 = fma2(f2, pack2(-1.f, -1.f), v);
                                 sums[j >> 3] = add2(sums[j >> 3], f2);
                                 rests[j >> 3] = add2(rests[j >> 3], r2);
                                 const float2 r = unpack2(r2);

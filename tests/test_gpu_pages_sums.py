@@ -92,3 +92,25 @@ def test_one_key_that_outweighs_many(below, ones, n_kv, new, past, bound):
     got = c.attend(first_element(new, 40, 128), Batch([new], [past]), 0.0, 0, scale=1.0)[at].double()
     off = ((got - want).abs() / want).max().item()
     assert off <= bound, off
+
+
+def half_steps(got, want):
+    """the largest difference, in half steps of got's type at want"""
+    u = torch.finfo(got.dtype).eps / 2
+    return ((got.double() - want).abs() / (2.0 ** want.abs().log2().floor() * u)).max().item()
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+@pytest.mark.parametrize("below", [2.0, 6.0, 9.0])
+def test_f16_prompts_round_once(below, cache):
+    """Probabilities enter f16 prompts in one f16 part, half a step of 2^-11 off at most, and the divisor is their sum: the weights of one key and of all others, at most a
+    quarter multiplied, are off by 2^-11 against each other, over values at most 1 apart: 1/4 half step of results from 1 to 2.  27 units of 128 keys, each cut off by
+    1.9e-6: 0.1 half steps.  With the result's own rounding 1.35."""
+    n_kv, new, past = 8, 512, 3000
+    scores, values = one_beside_many(below, False, new + past, n_kv, 128)
+    if cache == F8:
+        values = eighths(3, new + past, n_kv, 128)
+    c = filled(scores, values, 64, cache)
+    at, want = some_rows(scores, values, new, past, 40)
+    off = half_steps(c.attend(first_element(new, 40, 128, torch.float16), Batch([new], [past]), 0.0, 0, scale=1.0)[at], want)
+    assert off <= 1.35, off
