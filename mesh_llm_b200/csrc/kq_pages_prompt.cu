@@ -35,7 +35,9 @@ constexpr uint32_t COL_S = 0, COL_O = 256;
 // parts that O is made of, in O's steps and cut off as O's are: what a step loses there cancels where it is divided by, and where it loses nothing, neither
 // does the sum.  Relative error with positive values, 512 rows of 40 heads behind 3000 keys: 3.6e-6 where all weigh alike, at most 8.1e-6 where one outweighs
 // the others (every six units alone 2.0e-5); values of either sign: 1.1e-6.  Four units instead of six: 2.3e-6 for 5 % of the time.
-constexpr int FLUSH = 6;
+// Results of 16 bits put theirs aside for the same reason, when the loss nears an eighth of their half step (f16 32 units, bf16 128): without, 60000 keys cost
+// an f16 result up to 4.7 half steps.
+template <typename T> constexpr int FLUSH = std::is_same<T, float>::value ? 6 : std::is_same<T, __half>::value ? 32 : 128;
 constexpr float DOMINATED = 12.f;
 // Probabilities are worked out under 2^(m - PEAK), m the row's maximum when it last moved, and m moves when it would grow by more than GROWTH: they
 // stay below 2^(PEAK + GROWTH), and f16's smallest step of 2^-24 is 2^-35 of the largest.  (6 and 8: 60000 keys of e^-14 beside one of 1, 1.06e-5 off instead of 3.5e-6.)
@@ -628,13 +630,16 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             float *aside = a.part + (int64_t)gridDim.x * 2 * R * (HD + 2) + (int64_t)blockIdx.x * R * HD + 4 * (128 * half + row);
             int joined = 0;     // units in O since it was put aside
             float last_l = 0.f; // what the last one added to l
-            float m = -INFINITY, l = 0.f, l_sum = 0.f, m_sum = -INFINITY; // l_sum: of what was put aside; m_sum: the maximum that it goes by
+            float m = -INFINITY, l = 0.f;
+            float2 put = make_float2(-INFINITY, 0.f); // of what was put aside: the maximum that it goes by, and its l
+            // bf16, which seldom puts anything aside, keeps it in memory (2048 rows at 6144: 321 us, in registers 331, never 317; f16 421 and 410)
+            auto put_at = [&] { return reinterpret_cast<float2 *>(a.part + (int64_t)gridDim.x * R * (2 * (HD + 2) + HD)) + (int64_t)blockIdx.x * R + 128 * half + row; };
             // the row's O so far: what the tensor cores have summed and what was put aside before; as 32 columns a time
-            auto total = [&](int k, uint32_t *o) {
+            auto total = [&](int k, uint32_t *o, float2 put) {
                 tmem_ld32(to + 32 * k, o);
                 tmem_ld_wait();
-                if (PS == 2 && m_sum != -INFINITY) {
-                    const float f = ex2(m_sum - m);
+                if (put.x != -INFINITY) {
+                    const float f = ex2(put.x - m);
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         const float4 v = *reinterpret_cast<const float4 *>(aside + (8 * k + j / 4) * (4 * R));
@@ -654,11 +659,12 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 const int key0 = w.keys.x + (w.ub + i) * BK;
                 wait(sh.s_ready[half], units & 1, 10);
                 after_sync(); // S was issued behind the products before: O is at rest
-                if (PS == 2 && __any_sync(0xffffffffu, joined == FLUSH || (last_l > 0.f && l > DOMINATED * last_l))) {
+                if (BF ? i > 0 && i % FLUSH<T> == 0 : joined == FLUSH<T> || (PS == 2 && __any_sync(0xffffffffu, last_l > 0.f && l > DOMINATED * last_l))) {
+                    if (BF && i > FLUSH<T>) put = *put_at();
 #pragma unroll
                     for (int k = 0; k < HD / 32; k++) {
                         uint32_t o[32];
-                        total(k, o);
+                        total(k, o, put);
 #pragma unroll
                         for (int j = 0; j < 32; j += 4)
                             *reinterpret_cast<uint4 *>(aside + (8 * k + j / 4) * (4 * R)) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
@@ -667,10 +673,14 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         if (!*abort) tmem_st32(to + 32 * k, o);
                     }
                     tmem_st_wait();
-                    l_sum = l + (m_sum != -INFINITY ? l_sum * ex2(m_sum - m) : 0.f);
+                    put.y = l + (put.x != -INFINITY ? put.y * ex2(put.x - m) : 0.f);
+                    put.x = m;
                     l = 0.f;
-                    m_sum = m;
                     joined = 0;
+                    if (BF) {
+                        *put_at() = put;
+                        put = make_float2(-INFINITY, 0.f);
+                    }
                 }
                 joined++;
                 const bool masked = blocks != 0xff || key0 + BK - 1 > lim_lo || (a.window > 0 && key0 <= lim_hi - a.window);
@@ -793,7 +803,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             // ---- results
             wait(sh.o_done, pieces & 1, 12);
             after_sync();
-            if (PS == 2 && m_sum != -INFINITY) l = fmaf(l_sum, ex2(m_sum - m), l);
+            if (BF && w.take > FLUSH<T>) put = *put_at();
+            if (put.x != -INFINITY) l = fmaf(put.y, ex2(put.x - m), l);
             const bool whole = w.ub == 0 && w.take == w.n_units, ok = my_row_ok && !*abort;
             const float inv = m == -INFINITY ? 0.f : whole ? 1.f / l : 1.f; // a row that saw nothing is 0
             // 32 columns a time through the warp's part of the queries' room, so that a store writes whole lines of 4 rows
@@ -809,7 +820,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll 1
             for (int k = 0; k < HD / 32; k++) {
                 uint32_t o[32];
-                total(k, o);
+                total(k, o, put);
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -948,7 +959,7 @@ int kq_pages_error_fetch() {
     return v;
 }
 
-size_t kq_pages_prompt_scratch(int hd) { return META_BYTES + (size_t)kq_sm_count() * R * (2 * (hd + 2) + hd) * sizeof(float); } // two slots of a CTA, and what it puts aside
+size_t kq_pages_prompt_scratch(int hd) { return META_BYTES + (size_t)kq_sm_count() * R * (2 * (hd + 2) + hd + 2) * sizeof(float); } // two slots of a CTA, and what it puts aside
 
 b200_status kq_pages_prompt(KqAttnArgs a, bool f8, int hd, uint8_t *scratch, cudaStream_t st) {
     const int ctas = kq_sm_count();

@@ -114,3 +114,17 @@ def test_f16_prompts_round_once(below, cache):
     at, want = some_rows(scores, values, new, past, 40)
     off = half_steps(c.attend(first_element(new, 40, 128, torch.float16), Batch([new], [past]), 0.0, 0, scale=1.0)[at], want)
     assert off <= 1.35, off
+
+
+@pytest.mark.parametrize("dtype, past, bound", [(torch.float16, 60000, 1.75), (torch.bfloat16, 150000, 1.45)])
+@pytest.mark.parametrize("below", [14.0, 11.0, 0.0])
+def test_long_rows_of_16_bits(below, dtype, past, bound):
+    """A CTA sums hundreds of units of 128 keys, each cut off by 1.9e-6 of what it joins: by 32 of them, f16, or 128, bf16, at most.  In half steps of results from 1 to
+    2: f16 0.12 and, as probabilities are rounded, 1/2 at most (1/4 of the test above, twice over for sums of unlike units); bf16 2 x 0.06, its probabilities and their sum
+    2 x 2^-11 x 2^7 = 0.12 and as much again for the units', the cubic 2 x 0.02.  With the result's own rounding 1.75 and 1.45."""
+    n_kv, new = 4, 1280
+    scores, values = one_beside_many(below, False, new + past, n_kv, 128)
+    c = filled(scores, values, 64, torch.float16)
+    at, want = some_rows(scores, values, new, past, 40)
+    off = half_steps(c.attend(first_element(new, 40, 128, dtype), Batch([new], [past]), 0.0, 0, scale=1.0)[at], want)
+    assert off <= bound, off
