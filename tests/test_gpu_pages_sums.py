@@ -59,7 +59,7 @@ def test_sums_that_lose_nothing(weight, hd, cache):
 
 def some_rows(scores, values, new, past, n_head):
     """rows and what they are, from the definition in 64 bits: the queries are alike, so the heads of a KV head are too"""
-    at = sorted({0, 1, new // 2, new - 1})
+    at = sorted({0, min(1, new - 1), new // 2, new - 1})
     out = []
     for r in at:
         n = past + r + 1
@@ -127,4 +127,26 @@ def test_long_rows_of_16_bits(below, dtype, past, bound):
     c = filled(scores, values, 64, torch.float16)
     at, want = some_rows(scores, values, new, past, 40)
     off = half_steps(c.attend(first_element(new, 40, 128, dtype), Batch([new], [past]), 0.0, 0, scale=1.0)[at], want)
+    assert off <= bound, off
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+@pytest.mark.parametrize("dtype, bound", [(torch.float32, 256.0), (torch.float16, 1.2), (torch.bfloat16, 1.45)])
+def test_steps_of_long_rows(dtype, bound, cache):
+    """120 sequences over the pages of one, so that a CTA sums an item of 131072 keys alone, 2048 steps a warp.  f32: each step is added with a rounding of 2^-24 at
+    most, of O and of the divisor: four times the square root of 2 x 2048, 256 half steps.  f16: both parts, the same 256 half steps of f32 are 1/32 of f16's: with the
+    result's own rounding and the second parts' 1.2.  bf16: the tensor cores add up a warp's steps over f16 pages, 16 products a step cut off by 2^-26 each: 4.9e-4, an eighth of a half
+    step of results from 1 to 2, twice that where they are near 2; probabilities 2 x 2^-11 x 2^7 / 2; 1.45."""
+    n, n_kv, n_seq = 131072, 4, 120
+    g = torch.Generator("cuda").manual_seed(4)
+    scores = -12 + torch.randn((n, n_kv), generator=g, device="cuda")
+    scores[0] = 0
+    values = eighths(5, n, n_kv, 128)
+    c = filled(scores, values, 256, cache)
+    k = c.rows(0, n)[0][..., 0]  # the scores as the pages have them
+    c.table = c.table.expand(n_seq, -1).contiguous()
+    _, want = some_rows(k, values, 1, n - 1, 8)
+    q = first_element(n_seq, 8, 128, dtype)
+    got = c.attend(q, Batch([1] * n_seq, [n - 1] * n_seq), 0.0, 0, scale=1.0)
+    off = half_steps(got, want.expand(n_seq, -1, -1))
     assert off <= bound, off
