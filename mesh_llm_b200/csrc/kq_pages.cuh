@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 
 constexpr int KQ_PAGE_BLOCK = 16;
+constexpr int64_t KQ_MOST_ELEMENTS = (int64_t)1 << 48; // of a pool or of a call's rows with what lies between them: more than any device holds
 
 struct KqPages {
     uint8_t *k, *v;
@@ -33,7 +34,7 @@ struct KqTurns { // turns per position of each rotated pair in units of 2^-64; o
 
 // checks of a b200_kv_pages and its batch that need no device memory (kq_pages_append.cu)
 b200_status kq_pages_check(const char *who, const b200_kv_pages *c, const b200_page_batch *b, KqPages *out, KqBatch *batch);
-b200_status kq_rows_check(const char *who, const char *what, const void *p, uint32_t type, int64_t stride, int64_t width);
+b200_status kq_rows_check(const char *who, const char *what, const void *p, uint32_t type, int64_t rows, int64_t stride, int64_t width);
 KqTurns kq_turns(float theta, int neox, int hd);
 
 #ifdef __CUDACC__

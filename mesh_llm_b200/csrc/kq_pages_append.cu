@@ -17,6 +17,7 @@
 
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -300,7 +301,7 @@ b200_status kq_pages_check(const char *who, const b200_kv_pages *c, const b200_p
     KQ_REQUIRE(c->k && c->v && ((((uintptr_t)c->k | (uintptr_t)c->v)) & 15) == 0, "%s: page pools must be given and 16-byte aligned", who);
     KQ_REQUIRE(!f8 || (c->k_scale && c->v_scale && (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) == 0), "%s: e4m3 pages need their scales", who);
     const int64_t page = (int64_t)c->n_kv * c->page_size * c->head_dim, es = f8 ? 1 : 2, stride = c->page_stride ? c->page_stride : page;
-    KQ_REQUIRE(stride >= page && stride * es % 16 == 0 && stride <= ((int64_t)1 << 36), "%s: page stride %lld (at least a page of %lld elements, a multiple of 16 bytes)", who, (long long)stride,
+    KQ_REQUIRE(stride >= page && stride * es % 16 == 0 && stride <= KQ_MOST_ELEMENTS / c->n_pages && stride <= ((int64_t)1 << 36), "%s: page stride %lld (at least a page of %lld elements, a multiple of 16 bytes)", who, (long long)stride,
                (long long)page);
     KQ_REQUIRE(b->n_seq >= 0 && b->rows >= 0 && b->rows <= 0x3fffffff, "%s: %d sequences, %lld rows", who, b->n_seq, (long long)b->rows);
     KQ_REQUIRE(b->n_seq == 0 || (b->row_start && b->pos0 && (b->table || b->table_len == 0)), "%s: row starts, positions and page table required", who);
@@ -313,9 +314,11 @@ b200_status kq_pages_check(const char *who, const b200_kv_pages *c, const b200_p
     return B200_OK;
 }
 
-b200_status kq_rows_check(const char *who, const char *what, const void *p, uint32_t type, int64_t stride, int64_t width) {
+b200_status kq_rows_check(const char *who, const char *what, const void *p, uint32_t type, int64_t rows, int64_t stride, int64_t width) {
     KQ_REQUIRE(type == B200_TYPE_F32 || type == B200_TYPE_F16 || type == B200_TYPE_BF16, "%s: %s of type %u (f32, f16 or bf16)", who, what, type);
     const int64_t es = type == B200_TYPE_F32 ? 4 : 2;
+    // products of rows and strides stay far from 64 bits
+    KQ_REQUIRE(stride <= KQ_MOST_ELEMENTS / std::max<int64_t>(rows, 1), "%s: %s of %lld rows, %lld elements apart", who, what, (long long)rows, (long long)stride);
     KQ_REQUIRE(p && ((uintptr_t)p & 15) == 0 && stride >= width && stride * es % 16 == 0, "%s: %s must be 16-byte aligned rows, %lld elements or more apart", who, what, (long long)width);
     return B200_OK;
 }
@@ -328,8 +331,8 @@ extern "C" b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b2
     KQ_REQUIRE(theta >= 0.f && isfinite(theta), "kv_pages_append: rotation base %g", theta);
     if (b.rows == 0 || b.n_seq == 0) return B200_OK;
     const int64_t width = (int64_t)c.n_kv * cache->head_dim;
-    KQ_TRY(kq_rows_check("kv_pages_append", "keys", k, type, k_stride, width));
-    KQ_TRY(kq_rows_check("kv_pages_append", "values", v, type, v_stride, width));
+    KQ_TRY(kq_rows_check("kv_pages_append", "keys", k, type, b.rows, k_stride, width));
+    KQ_TRY(kq_rows_check("kv_pages_append", "values", v, type, b.rows, v_stride, width));
     const Rows r{k, v, k_stride, v_stride};
     const KqTurns turns = kq_turns(theta, neox, cache->head_dim);
     const bool f8 = cache->type == B200_TYPE_F8_E4M3;

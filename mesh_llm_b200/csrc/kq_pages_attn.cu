@@ -628,8 +628,8 @@ b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_bat
     KQ_REQUIRE(window >= 0 && window <= (1 << 30) && max_rows >= 0, "attention_pages: window %d, rows %d", window, max_rows);
     if (a.b.rows == 0 || a.b.n_seq == 0) return B200_OK;
     const int hd = cache->head_dim;
-    KQ_TRY(kq_rows_check("attention_pages", "queries", q, type, q_stride, (int64_t)n_head * hd));
-    KQ_TRY(kq_rows_check("attention_pages", "results", out, type, out_stride, (int64_t)n_head * hd));
+    KQ_TRY(kq_rows_check("attention_pages", "queries", q, type, a.b.rows, q_stride, (int64_t)n_head * hd));
+    KQ_TRY(kq_rows_check("attention_pages", "results", out, type, a.b.rows, out_stride, (int64_t)n_head * hd));
     KQ_REQUIRE(scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= b200_attention_pages_scratch_bytes(cache, n_head, max_rows),
                "attention_pages: scratch of %zu bytes, 16-byte aligned, required", b200_attention_pages_scratch_bytes(cache, n_head, max_rows));
     const int64_t es = type == B200_TYPE_F32 ? 4 : 2, width = (int64_t)n_head * hd * es, apart = (const uint8_t *)out - (const uint8_t *)q, row = q_stride * es;
