@@ -304,13 +304,15 @@ typedef struct b200_page_batch {
  * (where it holds earlier positions, whose codes are rescaled) and what the largest new value asks for.  A value beyond the
  * page type's range becomes the largest one; a NaN in v becomes 0 there and NaN at its place in the token's k, so
  * that exactly the queries that see the token give NaN.  No block of 16 positions may be written twice in one call (two
- * sequences, or two table entries, that name one page): which of them it then holds is not defined.              */
+ * sequences, or two table entries, that name one page): which of them it then holds is not defined.  Pools, scales, k and v must
+ * not lie over one another (pages of keys and values may take turns in one allocation). */
 B200_API b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type,
                                           const void *k, int64_t k_stride, const void *v, int64_t v_stride, float theta,
                                           int32_t neox, void *stream);
 /* Causal attention of the batch's rows over their sequences' pages: head h of a row at position p sees positions
  * p - window + 1 .. p (window 0: from 0 on; at most 2^30) that are there, of KV head h / (n_head / n_kv); a row that sees none is 0.
- * q, out (which must not overlap): [rows][n_head][head_dim] of type f32, f16 or bf16, q_stride and out_stride elements between rows, 16-byte aligned;
+ * q, out: [rows][n_head][head_dim] of type f32, f16 or bf16, q_stride and out_stride elements between rows, 16-byte aligned (out and scratch
+ * lie over no other buffer of the call);
  * the queries are rotated on the way in (theta 0: as they come).  scale 0: 1 / sqrt(head_dim).  max_rows: the most rows of a
  * sequence as far as the caller knows; it picks the kernels, any value is right.  f32: queries and probabilities enter
  * the products in two f16 parts (in prompts what a product loses goes by the sum that it joins: up to 1e-5 of the row's largest

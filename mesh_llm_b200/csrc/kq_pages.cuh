@@ -36,6 +36,17 @@ struct KqTurns { // turns per position of each rotated pair in units of 2^-64; o
 b200_status kq_pages_check(const char *who, const b200_kv_pages *c, const b200_page_batch *b, KqPages *out, KqBatch *batch);
 b200_status kq_rows_check(const char *who, const char *what, const void *p, uint32_t type, int64_t rows, int64_t stride, int64_t width);
 KqTurns kq_turns(float theta, int neox, int hd);
+// memory from the first byte of a buffer to behind its last
+struct KqSpan {
+    const char *what = "";
+    uintptr_t from = 0, to = 0;
+    KqSpan() {}
+    KqSpan(const char *what, const void *p, int64_t bytes) : what(what), from((uintptr_t)p), to(from + bytes) {}
+    bool over(const KqSpan &x) const { return from < x.to && x.from < to; }
+};
+inline KqSpan kq_rows_span(const char *what, const void *p, int64_t es, int64_t rows, int64_t stride, int64_t width) { return KqSpan(what, p, ((rows - 1) * stride + width) * es); }
+// the cache's pools (and scales) against a buffer of the call
+b200_status kq_pages_apart(const char *who, const b200_kv_pages *c, const KqSpan &x);
 
 #ifdef __CUDACC__
 // cos and sin of pos * f turns, f in units of 2^-64: the product's low 64 bits are the angle within its turn, to 2^-53 of f at least (in 32 bits the

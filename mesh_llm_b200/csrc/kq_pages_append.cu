@@ -323,6 +323,42 @@ b200_status kq_rows_check(const char *who, const char *what, const void *p, uint
     return B200_OK;
 }
 
+namespace {
+int pool_spans(const b200_kv_pages *c, KqSpan *out) { // keys, values and, for e4m3, their scales
+    const bool f8 = c->type == B200_TYPE_F8_E4M3;
+    const int64_t page = (int64_t)c->n_kv * c->page_size * c->head_dim, scales = c->n_pages * c->n_kv * (c->page_size / KQ_PAGE_BLOCK) * (int64_t)sizeof(float);
+    out[0] = kq_rows_span("the pool of keys", c->k, f8 ? 1 : 2, c->n_pages, c->page_stride ? c->page_stride : page, page);
+    out[1] = kq_rows_span("the pool of values", c->v, f8 ? 1 : 2, c->n_pages, c->page_stride ? c->page_stride : page, page);
+    if (!f8) return 2;
+    out[2] = KqSpan("the scales of keys", c->k_scale, scales);
+    out[3] = KqSpan("the scales of values", c->v_scale, scales);
+    return 4;
+}
+// what append writes must not lie over one another; pages of keys and values may take turns in one allocation
+b200_status pools_apart(const char *who, const b200_kv_pages *c) {
+    KqSpan pool[4];
+    const int n = pool_spans(c, pool);
+    for (int i = 0; i < n; i++)
+        for (int j = i + 1; j < n; j++) {
+            if (!pool[i].over(pool[j])) continue;
+            bool turns = false;
+            if (j == 1 && c->page_stride) {
+                const uintptr_t es = n == 4 ? 1 : 2, page = (uintptr_t)c->n_kv * c->page_size * c->head_dim * es, stride = (uintptr_t)c->page_stride * es;
+                const uintptr_t apart = (pool[0].from < pool[1].from ? pool[1].from - pool[0].from : pool[0].from - pool[1].from) % stride;
+                turns = apart >= page && apart + page <= stride;
+            }
+            KQ_REQUIRE(turns, "%s: %s over %s", who, pool[i].what, pool[j].what);
+        }
+    return B200_OK;
+}
+} // namespace
+
+b200_status kq_pages_apart(const char *who, const b200_kv_pages *c, const KqSpan &x) {
+    KqSpan pool[4];
+    for (int i = 0, n = pool_spans(c, pool); i < n; i++) KQ_REQUIRE(!x.over(pool[i]), "%s: %s over %s", who, x.what, pool[i].what);
+    return B200_OK;
+}
+
 extern "C" b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b200_page_batch *batch, uint32_t type, const void *k, int64_t k_stride,
                                             const void *v, int64_t v_stride, float theta, int32_t neox, void *stream) {
     KqPages c;
@@ -333,6 +369,10 @@ extern "C" b200_status b200_kv_pages_append(const b200_kv_pages *cache, const b2
     const int64_t width = (int64_t)c.n_kv * cache->head_dim;
     KQ_TRY(kq_rows_check("kv_pages_append", "keys", k, type, b.rows, k_stride, width));
     KQ_TRY(kq_rows_check("kv_pages_append", "values", v, type, b.rows, v_stride, width));
+    const int64_t es = type == B200_TYPE_F32 ? 4 : 2;
+    KQ_TRY(pools_apart("kv_pages_append", cache));
+    KQ_TRY(kq_pages_apart("kv_pages_append", cache, kq_rows_span("new keys", k, es, b.rows, k_stride, width)));
+    KQ_TRY(kq_pages_apart("kv_pages_append", cache, kq_rows_span("new values", v, es, b.rows, v_stride, width)));
     const Rows r{k, v, k_stride, v_stride};
     const KqTurns turns = kq_turns(theta, neox, cache->head_dim);
     const bool f8 = cache->type == B200_TYPE_F8_E4M3;

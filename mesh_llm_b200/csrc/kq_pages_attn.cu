@@ -636,6 +636,11 @@ b200_status b200_attention_pages(const b200_kv_pages *cache, const b200_page_bat
     const int64_t in_row = ((apart % row) + row) % row; // where results begin in a row of queries, if both are parts of rows as long
     KQ_REQUIRE(apart >= (a.b.rows - 1) * row + width || -apart >= (a.b.rows - 1) * out_stride * es + width || (q_stride == out_stride && in_row >= width && in_row + width <= row),
                "attention_pages: results over queries");
+    const KqSpan results = kq_rows_span("results", out, es, a.b.rows, out_stride, (int64_t)n_head * hd);
+    const KqSpan room("scratch", scratch, b200_attention_pages_scratch_bytes(cache, n_head, max_rows));
+    KQ_TRY(kq_pages_apart("attention_pages", cache, results));
+    KQ_TRY(kq_pages_apart("attention_pages", cache, room));
+    KQ_REQUIRE(!room.over(results) && !room.over(kq_rows_span("", q, es, a.b.rows, q_stride, (int64_t)n_head * hd)), "attention_pages: scratch over results or queries");
     a.q = q;
     a.out = out;
     a.q_stride = q_stride;

@@ -59,3 +59,64 @@ def test_strides_whose_products_pass_64_bits(stride):
 def test_pools_whose_size_passes_64_bits():
     for n, stride in ((0x7fffffff, 1 << 36), (1 << 20, 1 << 30)):
         assert append(cache(n_pages=n, page_stride=stride)) == -1 and attend(cache(n_pages=n, page_stride=stride)) == -1
+
+
+PAGE = 2 * 16 * 128  # elements of a page
+
+
+def test_results_and_scratch_over_the_cache():
+    for type, es in ((capi.TYPE_F16, 2), (capi.TYPE_F8_E4M3, 1)):
+        c = cache(type)
+        for pool in ("k_pool", "v_pool"):
+            at = PLACES[pool]
+            for out in (at, at + 4 * PAGE * es - 16, at - 3 * 4096 + 16):
+                assert attend(c, out=out) == -1, (pool, out - at)
+                assert attend(c, scratch=out) == -1
+            assert attend(c, out=at + 4 * PAGE * es) == THROUGH and attend(c, out=at - 3 * 4096) == THROUGH
+    c = cache(capi.TYPE_F8_E4M3)
+    for scales in ("ks", "vs"):
+        assert attend(c, out=PLACES[scales]) == -1 and attend(c, scratch=PLACES[scales]) == -1
+    assert attend(out=PLACES["scratch"]) == -1 and attend(q=PLACES["scratch"] + 4096) == -1
+    wide = cache(page_stride=3 * PAGE)
+    assert attend(wide, out=PLACES["k_pool"] + 3 * 3 * PAGE * 2 + 2 * PAGE - 16) == -1
+    assert attend(wide, out=PLACES["k_pool"] + (3 * 3 + 1) * PAGE * 2) == THROUGH
+
+
+def test_append_into_pools_that_overlap():
+    k = PLACES["k_pool"]
+    assert append(cache(v=k)) == -1 and append(cache(v=k + 2 * PAGE)) == -1 and append(cache(k=PLACES["v_pool"] + 8 * PAGE - 16)) == -1
+    assert append(cache(v=k + 2 * 4 * PAGE)) == THROUGH  # one behind the other
+    for first, second in ((k, k + 2 * PAGE), (k + 2 * PAGE, k)):  # in turn
+        assert append(cache(k=first, v=second, page_stride=2 * PAGE)) == THROUGH
+        assert append(cache(k=first, v=second, page_stride=2 * PAGE - 16)) == -1
+    assert append(cache(v=k + 2 * PAGE - 16, page_stride=2 * PAGE)) == -1
+    f8 = capi.TYPE_F8_E4M3
+    assert append(cache(f8, v_scale=PLACES["ks"])) == -1 and append(cache(f8, v_scale=PLACES["ks"] + 28)) == -1 and append(cache(f8, v_scale=PLACES["ks"] + 32)) == THROUGH
+    assert append(cache(f8, k_scale=k)) == -1
+    assert attend(cache(v=k)) == THROUGH  # attention only reads them
+
+
+def test_append_of_rows_that_lie_in_the_cache():
+    for rows in ("k", "v"):
+        for pool in ("k_pool", "v_pool"):
+            assert append(**{rows: PLACES[pool] + 4096}) == -1
+    assert append(v=PLACES["k"]) == THROUGH  # both only read
+
+
+def test_what_is_refused_is_refused_for_itself():
+    """the refusals of one argument each, of a call that is let through without it"""
+    from tests.test_pages_cpu import BAD_BATCH, BAD_CACHE
+
+    for bad in BAD_CACHE:
+        d = {**dict(k_scale=None, v_scale=None), **bad}
+        assert append(cache(**d)) == -1 and attend(cache(**d)) == -1, bad
+    for bad in BAD_BATCH:
+        assert append(b=batch(**bad)) == -1 and attend(b=batch(**bad)) == -1, bad
+    for bad in (dict(type=12), dict(k=None), dict(v=PLACES["v"] + 4), dict(ks=255), dict(vs=258), dict(ks=-256)):
+        assert append(**bad) == -1, bad
+    for bad in (dict(type=8), dict(q=None), dict(out=None), dict(out=PLACES["out"] + 8), dict(qs=1023), dict(os=1026), dict(most=-1), dict(scratch=None), dict(scratch=PLACES["scratch"] + 8)):
+        assert attend(**bad) == -1, bad
+    q = PLACES["q"]
+    for out, stride in ((q, 1024), (q + 16, 1024), (q + 2 * 4096 + 4080, 1024), (q - 2 * 4096 - 4080, 1024), (q + 4096, 2048), (q - 4096, 2048)):
+        assert attend(out=out, os=stride) == -1
+    assert attend(qs=2048, os=2048, out=q + 4096) == THROUGH  # parts of the same rows
