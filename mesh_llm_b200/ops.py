@@ -287,9 +287,14 @@ def _pages_call(rows, k_pages, v_pages, table, row_start, pos0, k_scale, v_scale
     type_ = _PAGE_TYPES.get(dtype)
     if type_ is None or v_pages.dtype is not dtype:
         raise ValueError(f"pages of {dtype} / {v_pages.dtype}: float16 or float8_e4m3fn expected")
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride:
+    if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError("pages: two pools [n_pages, n_kv, page_size, hd] of one shape and layout expected")
     n_pages, n_kv, size, hd = shape
+    if stride[1:] != (size * hd, hd, 1) or v_pages.stride() != stride:  # what a dimension of length 1 has for its stride says nothing
+        stride, v_stride = ([d if n == 1 else x for n, x, d in zip(shape, p.stride(), (n_kv * size * hd, size * hd, hd, 1))] for p in (k_pages, v_pages))
+        if v_stride != stride:
+            raise ValueError("pages: two pools [n_pages, n_kv, page_size, hd] of one shape and layout expected")
+        stride = tuple(stride)
     if n_pages and (stride[1:] != (size * hd, hd, 1) or n_pages > 1 and stride[0] < n_kv * size * hd):
         raise ValueError("pages: each page must be contiguous and its own")
     dev = rows.get_device()

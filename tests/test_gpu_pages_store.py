@@ -111,3 +111,19 @@ def test_every_code_times_its_scale_is_an_f16_number(exponent):
         q = torch.zeros((n, 1, hd), device="cuda")
         got = c.attend(q, Batch([n], [0]), 0.0, 0, window=1, max_rows=most)
         assert torch.equal(got.double(), values)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, F8])
+def test_pools_of_one_head_as_views(dtype):
+    """[pages, positions, 1, hd] seen as [pages, 1, positions, hd]: the memory of a pool of one KV head"""
+    c, d = (Cache(2, 60, 32, 1, 64, dtype, seed=53) for _ in "cd")
+    byte = torch.uint8 if dtype == F8 else torch.int16
+    d.k, d.v = (x.view(byte).reshape(c.n_pages, 32, 1, 64).permute(0, 2, 1, 3).view(dtype) for x in (d.k, d.v))
+    assert d.k.stride(1) == 64
+    b = Batch([20, 3], [0, 50])
+    k, v, q = randn(56, b.rows, 1, 64, torch.float32), randn(57, b.rows, 1, 64, torch.float32), randn(58, b.rows, 6, 64, torch.float32)
+    for x in (c, d):
+        x.append(k, v, b, 1e4, 0)
+    assert torch.equal(c.k.view(byte), d.k.view(byte)) and torch.equal(c.v.view(byte), d.v.view(byte))
+    late = Batch([20, 0], [0, 0])  # the second sequence's earlier positions were never written
+    assert torch.equal(c.attend(q, late, 1e4, 0)[:20], d.attend(q, late, 1e4, 0)[:20])

@@ -120,3 +120,25 @@ def test_what_is_refused_is_refused_for_itself():
     for out, stride in ((q, 1024), (q + 16, 1024), (q + 2 * 4096 + 4080, 1024), (q - 2 * 4096 - 4080, 1024), (q + 4096, 2048), (q - 4096, 2048)):
         assert attend(out=out, os=stride) == -1
     assert attend(qs=2048, os=2048, out=q + 4096) == THROUGH  # parts of the same rows
+
+
+def test_strides_of_dimensions_of_length_one_say_nothing():
+    """pools of one KV head as views of [pages, positions, heads, hd], or of one page: what is left to refuse is that they are not on a GPU"""
+    import torch
+
+    from mesh_llm_b200 import ops
+
+    i = torch.zeros(2, dtype=torch.int32)
+    for n_pages, n_kv, good in ((4, 1, True), (1, 1, True), (1, 2, False), (4, 2, False)):
+        pool = torch.zeros((n_pages, 16, n_kv, 128), dtype=torch.float16).permute(0, 2, 1, 3)
+        x = torch.zeros((3, n_kv, 128))
+        with pytest.raises(ValueError, match="CUDA" if good else "its own"):
+            ops.kv_pages_append(x, x, pool, pool.clone(memory_format=torch.preserve_format), i[None, :1], i, i[:1], 1e4, 1)
+    one = torch.zeros((4, 2, 16, 128), dtype=torch.float16)[1:2]
+    other = torch.zeros((1, 2, 16, 128), dtype=torch.float16).as_strided((1, 2, 16, 128), (77, 2048, 128, 1))
+    x = torch.zeros((3, 2, 128))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.kv_pages_append(x, x, one, other, i[None, :1], i, i[:1], 1e4, 1)
+    with pytest.raises(ValueError, match="one shape and layout"):
+        big = torch.zeros((8, 2, 16, 128), dtype=torch.float16)
+        ops.kv_pages_append(x, x, big[::2], big[:4], i[None, :1], i, i[:1], 1e4, 1)
