@@ -142,3 +142,20 @@ def test_strides_of_dimensions_of_length_one_say_nothing():
     with pytest.raises(ValueError, match="one shape and layout"):
         big = torch.zeros((8, 2, 16, 128), dtype=torch.float16)
         ops.kv_pages_append(x, x, big[::2], big[:4], i[None, :1], i, i[:1], 1e4, 1)
+
+
+def test_waits_that_give_up_are_told_apart():
+    """a code of b200_check_device_waits names the paged kernels' wait: four bits of their own (every wait of theirs has a number below 16)"""
+    import os
+    import re
+
+    src = os.path.join(os.path.dirname(os.path.abspath(capi.__file__)), "csrc")
+    text = open(os.path.join(src, "kq_capi.cu")).read()
+    body = re.search(r"int kq_device_wait_errors\(\) \{(.*?)\n\}", text, re.S).group(1)
+    shifts = {}
+    for names, shift in re.findall(r"\(+((?:kq_\w+_error_fetch\(\)(?: \| )?)+)\)? << (\d+)\)", body):
+        for name in re.findall(r"kq_(\w+)_error_fetch", names):
+            shifts[name] = int(shift)
+    assert shifts["pages"] == 24 and [n for n, s in shifts.items() if s == 24] == ["pages"]
+    codes = [int(c) for c in re.findall(r"wait(?:_all)?\(sh\.[^;]*, (\d+)\)", open(os.path.join(src, "kq_pages_prompt.cu")).read())]
+    assert len(codes) >= 10 and 0 < min(codes) and max(codes) < 16
