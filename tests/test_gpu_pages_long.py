@@ -116,3 +116,59 @@ def test_attention_over_offsets_past_32_bits(cache, dtype):
         q = randn(45, new, 16, hd, dtype)
         got = ops.attention_pages(q, big[0], big[1], table, b.start, b.pos0, new, 1e6, 1, k_scale=big[2], v_scale=big[3])
         assert torch.equal(got, small.attend(q, b, 1e6, 1))
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+def test_prompts_captured_once_with_lengths_that_change(cache):
+    """a graph of append and attention follows the rows and positions that the device holds at its replay, prompts and steps in any place"""
+    n_head, n_kv, hd, rows = 10, 2, 128, 500
+    c, e = (Cache(4, 900, 32, n_kv, hd, cache, seed=41) for _ in "ce")
+    q, k, v = randn(46, rows, n_head, hd), randn(47, rows, n_kv, hd), randn(48, rows, n_kv, hd)
+    b = Batch([rows, 0, 0, 0], [0, 0, 0, 0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.append(k, v, b, 1e4, 1)
+        out = c.attend(q, b, 1e4, 1, max_rows=rows)
+    past = [0, 0, 0, 0]
+    for new in ([rows, 0, 0, 0], [1, 300, 2, 197], [1, 1, 350, 1], [0, 80, 1, 400], [3, 1, 1, 1], [90, 90, 90, 90]):
+        step = Batch(new, past)
+        b.start.copy_(step.start)
+        b.pos0.copy_(step.pos0)
+        out.zero_()
+        g.replay()
+        e.append(k[:step.rows], v[:step.rows], step, 1e4, 1)
+        assert torch.equal(out[:step.rows], e.attend(q[:step.rows], step, 1e4, 1, max_rows=rows))
+        assert (out[step.rows:] == 0).all()
+        close(out[:step.rows], attention(e, q[:step.rows], step, 1e4, 1))
+        past = [p + t for p, t in zip(past, new)]
+
+
+def test_prompts_on_streams_at_once():
+    c, b = filled([900], [300], 64, 2, 128, torch.float16, 1e4, 1), Batch([300], [900])
+    q = randn(49, 300, 16, 128, torch.bfloat16)
+    want = c.attend(q, b, 1e4, 1)
+    close(want, attention(c, q, b, 1e4, 1))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for i in range(30):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(c.attend(q, b, 1e4, 1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+def test_more_sequences_than_threads_and_more_heads_than_rows(cache):
+    """700 sequences of which some are prompts; 300 query heads on one KV head"""
+    new = [1 if i % 100 else 150 for i in range(700)]
+    past = [(37 * i) % 190 for i in range(700)]
+    c, b = filled(past, new, 16, 1, 64, cache, 1e4, 1), Batch(new, past)
+    q = randn(50, b.rows, 2, 64)
+    close(c.attend(q, b, 1e4, 1), attention(c, q, b, 1e4, 1))
+    for t in (1, 3, 40):
+        c, b = filled([500], [t], 32, 1, 128, cache, 1e4, 0), Batch([t], [500])
+        q = randn(51, t, 300, 128)
+        for most in (t, 0):
+            close(c.attend(q, b, 1e4, 0, max_rows=most), attention(c, q, b, 1e4, 0))
