@@ -32,9 +32,10 @@ constexpr uint32_t COL_S = 0, COL_O = 256;
 // f32: the tensor cores cut their sums off instead of rounding them: of a product what lies below 2^-25 of the sum that it joins, of a step's sum what lies
 // below its 24 bits.  So O and the row's sum of probabilities are put aside and added up in 32 bits every FLUSH units, and as soon as a unit has added less than
 // 1 / DOMINATED of what is there: what a unit of 128 keys loses is in proportion to what it joins, 1.9e-6 of that on average.  The sum is taken of the
-// parts that O is made of, in O's steps and cut off as O's are: what a step loses there cancels where it is divided by, and where it loses nothing, neither
-// does the sum.  Relative error with positive values, 512 rows of 40 heads behind 3000 keys: 3.6e-6 where all weigh alike, at most 8.1e-6 where one outweighs
-// the others (every six units alone 2.0e-5); values of either sign: 1.1e-6.  Four units instead of six: 2.3e-6 for 5 % of the time.
+// same probabilities in O's steps and cut off as often as O is, but not where a step joins nothing: what O loses to its 24 bits cancels on average where it is
+// divided by.  Relative error, 512 rows of 40 heads behind 3000 keys: values of either sign 1.1e-6; positive values 2.8e-6 where keys weigh alike, at most 8.0e-6
+// where one outweighs the others (every six units alone 2.0e-5), and less than 6e-7 where all weight is on one.  Five and four units instead of six: 1.0e-6 and
+// 0.9e-6 for 5 and 7 % of the time.
 // Results of 16 bits put theirs aside for the same reason, when the loss nears an eighth of their half step (f16 32 units, bf16 128): without, 60000 keys cost
 // an f16 result up to 4.7 half steps.
 template <typename T> constexpr int FLUSH = std::is_same<T, float>::value ? 6 : std::is_same<T, __half>::value ? 32 : 128;
@@ -759,7 +760,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                             if (PS == 1 && !BF) sums[j & 1] = add2(sums[j & 1], f2);
                             if (PS == 2) {
                                 const uint64_t r2 = fma2(f2, pack2(-1.f, -1.f), v);
-                                sums[j >> 3] = add2(sums[j >> 3], f2);
+                                sums[j >> 3] = add2(sums[j >> 3], v);
                                 rests[j >> 3] = add2(rests[j >> 3], r2);
                                 const float2 r = unpack2(r2);
                                 const uint32_t rest = h2(r.x, r.y);
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                             if (e) {
 #pragma unroll
                                 for (int g = 0; g < 4; g++)
-                                    if (fabsf(rest_sums[g]) >= l * 0x1p-25f) l = __fadd_rz(l, rest_sums[g]);
+                                    if (fabsf(rest_sums[g]) >= l * 0x1p-25f) l = __fadd_rz(l, rest_sums[g]) - rest_sums[g]; // their sum is in l already
                             }
                         }
                         if (!*abort) {

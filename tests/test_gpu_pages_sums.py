@@ -150,3 +150,21 @@ def test_steps_of_long_rows(dtype, bound, cache):
     got = c.attend(q, Batch([1] * n_seq, [n - 1] * n_seq), 0.0, 0, scale=1.0)
     off = half_steps(got, want.expand(n_seq, -1, -1))
     assert off <= bound, off
+
+
+@pytest.mark.parametrize("past", [1536, 8000])
+@pytest.mark.parametrize("cache", [torch.float16, F8])
+def test_f32_prompts_of_random_rows(cache, past):
+    """Relative 2-norm of the error of ordinary rows, whose values are of either sign.  O's steps are cut off to 24 bits, half a last bit each on average, and the divisor's are too;
+    what is left is the products' own cutting, 2^-26 of the sum for each of 768 keys at most and of either sign (0.5 sqrt(768) 2^-26 sqrt(1/3): 1.2e-7 for each part), the
+    spread of 192 cuts of up to 2^-23 (sqrt(192 / 12) 2^-23 x 2/3 as sums grow: 3.2e-7, O's and the divisor's: 4.5e-7), half of the bias where they do not match (96 x 2^-24 x 2/3 / 2 / 2: 9.5e-7),
+    and scores of 22 and 24 bits (2^-22 of up to 3: 7e-7 on a probability, over many keys 4e-7).  Together 1.2e-6."""
+    g = torch.Generator("cuda").manual_seed(6)
+    n_head, n_kv, new = 40, 8, 512
+    k, v = (torch.randn((new + past, n_kv, 128), generator=g, device="cuda") for _ in "kv")
+    c = Cache(1, new + past, 64, n_kv, 128, cache, seed=31)
+    c.append(k, v, Batch([new + past], [0]), 1e6, 1)
+    q, b = torch.randn((new, n_head, 128), generator=g, device="cuda"), Batch([new], [past])
+    want = attention(c, q, b, 1e6, 1)
+    off = ((c.attend(q, b, 1e6, 1).double() - want).norm() / want.norm()).item()
+    assert off <= 1.2e-6, off
