@@ -62,6 +62,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t *r) { T
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ float add_f16(float c, uint32_t h) { // c and the lower f16 of h
+    asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(c) : "h"((uint16_t)h), "f"(c));
+    return c;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -730,7 +734,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 }
                 const float sub = m == -INFINITY ? 0.f : m - PEAK;
                 hide_values(key0, seen);
-                uint64_t sums[2] = {0, 0}; // f32: of the steps of a chunk; else of all keys, in two runs
+                uint64_t sums[2] = {0, 0}; // f32: of the steps of a chunk; bf16: of all keys, in two runs
+                float rounded[4] = {0.f, 0.f, 0.f, 0.f}; // f16's
                 const float l_before = l;
                 uint32_t lo_even[PS == 2 ? 16 : 1];
                 const uint64_t crow2 = pack2(crow, crow), nsub2 = pack2(-sub, -sub);
@@ -753,13 +758,15 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                             if (BF) sums[j & 1] = add2(sums[j & 1], v);
                             const float2 p = unpack2(v);
                             hi[j] = h2(p.x, p.y);
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
-                            const uint64_t f2 = pack2(f.x, f.y);
                             // f16: the divisor is the sum of the weights as O has them, rounded, so that one weight's rounding is not the result's.  (Two parts
                             // as in f32 take 2048 rows at 6144 from 385 to 484 us, for results 1.01 instead of 1.13 half steps off.)
-                            if (PS == 1 && !BF) sums[j & 1] = add2(sums[j & 1], f2);
+                            if (PS == 1 && !BF) {
+                                rounded[j & 1] = add_f16(rounded[j & 1], hi[j]);
+                                rounded[2 + (j & 1)] = add_f16(rounded[2 + (j & 1)], hi[j] >> 16);
+                            }
                             if (PS == 2) {
-                                const uint64_t r2 = fma2(f2, pack2(-1.f, -1.f), v);
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
+                                const uint64_t r2 = fma2(pack2(f.x, f.y), pack2(-1.f, -1.f), v);
                                 sums[j >> 3] = add2(sums[j >> 3], v);
                                 rests[j >> 3] = add2(rests[j >> 3], r2);
                                 const float2 r = unpack2(r2);
@@ -798,7 +805,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 if (PS == 2) last_l = l - l_before;
                 else {
                     const float2 v = unpack2(add2(sums[0], sums[1]));
-                    l += v.x + v.y;
+                    l += BF ? v.x + v.y : (rounded[0] + rounded[1]) + (rounded[2] + rounded[3]);
                 }
             }
             // ---- results
