@@ -31,14 +31,15 @@ constexpr uint64_t LIMIT = 5 * KQ_WAIT_LIMIT_NS;
 constexpr uint32_t COL_S = 0, COL_O = 256;
 // f32: the tensor cores cut their sums off instead of rounding them: of a product what lies below 2^-25 of the sum that it joins, of a step's sum what lies
 // below its 24 bits.  So O and the row's sum of probabilities are put aside and added up in 32 bits every FLUSH units, and as soon as a unit has added less than
-// 1 / DOMINATED of what is there: what a unit of 128 keys loses is in proportion to what it joins, 1.9e-6 of that on average.  The sum is taken of the
-// same probabilities in O's steps and cut off as often as O is, but not where a step joins nothing: what O loses to its 24 bits cancels on average where it is
-// divided by.  Relative error, 512 rows of 40 heads behind 3000 keys: values of either sign 1.1e-6; positive values 2.8e-6 where keys weigh alike, at most 8.0e-6
-// where one outweighs the others (every six units alone 2.0e-5), and less than 6e-7 where all weight is on one.  Five and four units instead of six: 1.0e-6 and
-// 0.9e-6 for 5 and 7 % of the time.
+// 1 / DOMINATED of what is there: what a unit of 128 keys loses is in proportion to what it joins, 1.9e-6 of that on average.  The sum is taken in O's
+// steps and cut off as O is, first parts by adding so, second parts by CUT_HALF_BIT for a step where there are any of some weight: what O loses to its 24 bits
+// cancels on average where it is divided by.  Relative error, 512 rows of 40 heads behind 3000 keys: values of either sign 1.1e-6; positive values 2.7e-6
+// where keys weigh alike, at most 7.4e-6 where one outweighs the others (every six units alone 2.0e-5), less than 6e-7 where all weight is on one.  Five units
+// instead of six: 1.0e-6 for 5 % of the time.
 // Results of 16 bits put theirs aside for the same reason, when the loss nears an eighth of their half step (f16 32 units, bf16 128): without, 60000 keys cost
 // an f16 result up to 4.7 half steps.
 template <typename T> constexpr int FLUSH = std::is_same<T, float>::value ? 6 : std::is_same<T, __half>::value ? 32 : 128;
+constexpr float CUT_HALF_BIT = 4.3e-8f; // half a last bit relative to the value, over mantissas of 1 to 2 as they come: 2^-24 / (2 ln 2)
 constexpr float DOMINATED = 12.f;
 // Probabilities are worked out under 2^(m - PEAK), m the row's maximum when it last moved, and m moves when it would grow by more than GROWTH: they
 // stay below 2^(PEAK + GROWTH), and f16's smallest step of 2^-24 is 2^-35 of the largest.  (6 and 8: 60000 keys of e^-14 beside one of 1, 1.06e-5 off instead of 3.5e-6.)
@@ -743,10 +744,9 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                 for (int h64 = 0; h64 < 2; h64++) {
                     uint32_t hi[16], lo[PS == 2 ? 16 : 1];
-                    float rest_sums[4]; // of the second parts, by step
+                    float cuts = 0.f; // of the second parts' steps
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        uint64_t rests[2] = {0, 0};
                         const int c = 2 * h64 + e;
                         uint32_t(&x)[32] = s[c];
 #pragma unroll
@@ -765,12 +765,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                                 rounded[2 + (j & 1)] = add_f16(rounded[2 + (j & 1)], hi[j] >> 16);
                             }
                             if (PS == 2) {
-                                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[j]));
-                                const uint64_t r2 = fma2(pack2(f.x, f.y), pack2(-1.f, -1.f), v);
                                 sums[j >> 3] = add2(sums[j >> 3], v);
-                                rests[j >> 3] = add2(rests[j >> 3], r2);
-                                const float2 r = unpack2(r2);
-                                const uint32_t rest = h2(r.x, r.y);
+                                const uint32_t rest = h2_low(p.x, p.y, hi[j]);
                                 if (e == 0) lo_even[PS == 2 ? j : 0] = rest;
                                 else lo[PS == 2 ? j : 0] = rest;
                             }
@@ -779,16 +775,13 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                             for (int g = 0; g < 2; g++) {
                                 const float2 v = unpack2(sums[g]);
-                                l = __fadd_rz(l, v.x + v.y);
+                                const float sum = v.x + v.y;
+                                l = __fadd_rz(l, sum);
+                                // second parts are 2^-12 of the first at most, and there are none where a step's sum is one of f16 numbers (which leave low bits 0)
+                                if (sum >= l * 0x1p-13f && (__float_as_uint(sum) & 0x7ff)) cuts += CUT_HALF_BIT;
                                 sums[g] = 0;
-                                const float2 r = unpack2(rests[g]);
-                                rest_sums[2 * e + g] = r.x + r.y;
                             }
-                            if (e) {
-#pragma unroll
-                                for (int g = 0; g < 4; g++)
-                                    if (fabsf(rest_sums[g]) >= l * 0x1p-25f) l = __fadd_rz(l, rest_sums[g]) - rest_sums[g]; // their sum is in l already
-                            }
+                            if (e) l = fmaf(l, -cuts, l);
                         }
                         if (!*abort) {
                             tmem_st16(ts + 64 * h64 + 16 * e, hi);
