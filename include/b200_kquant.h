@@ -278,7 +278,8 @@ B200_API b200_status b200_attention_kv(const float *q, const void *k_cache, cons
  * contiguous caches above; the reference leaves this to its server).  Pools k and v: [n_pages][n_kv][page_size]
  * [head_dim], page_stride elements from one page to the next (0: dense), of type f16, or e4m3 with one scale per
  * aligned block of 16 positions and head, k_scale and v_scale [n_pages][n_kv][page_size / 16].  A scale is a power
- * of two from 2^-15 to 2^7, so code times scale is an f16 number.  head_dim 64 or 128, page_size a multiple of 16.
+ * of two from 2^-15 to 2^7, so code times scale is an f16 number.  head_dim 64 or 128, page_size a multiple of 16.  Append leaves
+ * finite values; who fills v otherwise must too, in every position that some row of a call sees (a row may see less than others).
  * A batch: row r of its `rows` rows belongs to the sequence s with row_start[s] <= r < row_start[s + 1] (ascending,
  * n_seq + 1 entries; rows no sequence owns are left alone) and stands at position pos0[s] + r - row_start[s];
  * table[s][i] is the page of positions i page_size .. of sequence s, table_len entries that are table_stride apart (together

@@ -10,10 +10,12 @@
 // B operand of O^T = V^T P^T.  Softmax in base 2, statistics in 32 bits.
 // A query row enters divided by the power of two that brings its largest element to [1, 2), so f16 neither overflows nor loses small
 // rows; f32 and f16 rows go in as two f16 parts (rotation makes an f16 query longer than f16), and so do their probabilities; the tensor cores
-// cut their sums off instead of rounding them, so those of one step (16 or 32 keys) are added to the row in 32-bit registers.
+// cut their sums off instead of rounding them, so those of one step (16 or 32 keys) are added to the row in 32-bit registers.  bf16 over f16 pages, whose
+// results have 8 bits, lets the tensor cores add up a warp's steps (131072 keys in one CTA, one of which outweighs the others: 1.08 half steps off).
 //
-// Bound by HBM: a position costs 2 hd codes per KV head and is read once.  f16 pages, 200 sequences of 60 to 6000 positions: 6.2 TB/s, 0.95 of a copy's
-// rate; e4m3 pages, half the bytes for as much arithmetic: 4.4 TB/s, where the instruction streams around the conversions count as much.  The units of
+// Bound by HBM: a position costs 2 hd codes per KV head and is read once.  Whole calls, joining launch included: f16 pages, 200 sequences of 60 to 6000
+// positions of 8 KV heads 6.2 TB/s, 0.95 of a copy's rate, 64 sequences of 4 KV heads 5.2; e4m3 pages, half the bytes for as much arithmetic, 200 sequences: 4.3 TB/s,
+// where the instruction streams around the conversions count as much.  The units of
 // all items are shared out evenly (kq_pages_sched.cuh), the four warps of a CTA take neighbouring positions and join their rows through shared memory at an item's end.
 #include "kq_pages_sched.cuh"
 

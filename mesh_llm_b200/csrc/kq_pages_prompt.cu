@@ -13,8 +13,8 @@
 // out-of-range coordinate; e4m3 pages arrive as raw rows by bulk copies and four warps turn them into the f16 tile of what they stand for.
 //
 // Bound, where items are long, by the tensor pipe (4 x 512 clocks for 256 rows x 128 keys at head_dim 128), the exponentials (16 a clock: 2 x 1024) and the
-// issue slots, all three near 2000 of the 3300 clocks that a unit takes; where they are short, by setting an item up (33 k clocks for a CTA's first, 27 k
-// for another).  4096 rows of 40 heads behind 12288 positions, bf16: 1.0 PFLOP/s.  Units are shared out evenly over one CTA per SM (kq_pages_sched.cuh).
+// issue slots, all three near 2000 of the 3300 clocks that a unit of bf16 takes; where they are short, by setting an item up (33 k clocks for a CTA's first, 27 k
+// for another).  4096 rows of 40 heads behind 12288 positions, bf16: 0.97 PFLOP/s (1240 us, under the power cap); f32 2130 us, f16 1580.  Units are shared out evenly over one CTA per SM (kq_pages_sched.cuh).
 // Every wait is bounded: on a time-out the kernel records an error, lets its copies land, frees its TMEM and returns.
 #include "kq_pages_sched.cuh"
 #include "kq_tc.cuh"
@@ -37,7 +37,7 @@ constexpr uint32_t COL_S = 0, COL_O = 256;
 // where keys weigh alike, at most 7.4e-6 where one outweighs the others (every six units alone 2.0e-5), less than 6e-7 where all weight is on one.  Five units
 // instead of six: 1.0e-6 for 5 % of the time.
 // Results of 16 bits put theirs aside for the same reason, when the loss nears an eighth of their half step (f16 32 units, bf16 128): without, 60000 keys cost
-// an f16 result up to 4.7 half steps.
+// an f16 result up to 5.0 half steps instead of 1.2, 150000 a bf16 result 2.1 instead of 1.03.
 template <typename T> constexpr int FLUSH = std::is_same<T, float>::value ? 6 : std::is_same<T, __half>::value ? 32 : 128;
 constexpr float CUT_HALF_BIT = 4.3e-8f; // half a last bit relative to the value, over mantissas of 1 to 2 as they come: 2^-24 / (2 ln 2)
 constexpr float DOMINATED = 12.f;
@@ -753,7 +753,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         for (int j = 0; j < 16; j++) {
                             uint64_t v = fma2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), crow2, nsub2);
                             // results of 8 bits: 3 of 8 exponentials on the FMA pipe, so that neither it nor the special-function unit decides alone
-                            // (4096 rows behind 12288 positions: 1509, 1480, 1460, 1437 us for 0, 1, 2, 3 of 8)
+                            // (4096 rows behind 12288 positions: 1509, 1480, 1460, 1437 us for 0, 1, 2, 3 of 8, when these were tried)
                             v = BF && j % 8 < POLY ? exp2_poly(v) : exp2_sfu(v);
                             if (BF) sums[j & 1] = add2(sums[j & 1], v);
                             const float2 p = unpack2(v);
