@@ -483,6 +483,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                 for (int j = 0; j < HD / 8; j++) *reinterpret_cast<uint4 *>(d + (j >> 3) * HALF + (j & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
+            __syncwarp();
             fence_async();
         };
         while (w.next(a)) {
@@ -655,6 +656,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         o[j + 3] = __float_as_uint(fmaf(v.w, f, __uint_as_float(o[j + 3])));
                     }
                 }
+                __syncwarp();
             };
             for (int i = 0; i < w.take; i++, units++) {
                 if ((i & 3) == 0) {
@@ -664,6 +666,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 const uint32_t blocks = (there >> (8 * (i & 3))) & 0xff;
                 const int key0 = w.keys.x + (w.ub + i) * BK;
                 wait(sh.s_ready[half], units & 1, 10);
+                __syncwarp(); // what reads and writes TMEM takes whole warps
                 after_sync(); // S was issued behind the products before: O is at rest
                 if (BF ? i > 0 && i % FLUSH<T> == 0 : joined == FLUSH<T> || (PS == 2 && __any_sync(0xffffffffu, last_l > 0.f && l > DOMINATED * last_l))) {
                     if (BF && i > FLUSH<T>) put = *put_at();
@@ -803,6 +806,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             }
             // ---- results
             wait(sh.o_done, pieces & 1, 12);
+            __syncwarp();
             after_sync();
             if (BF && w.take > FLUSH<T>) put = *put_at();
             if (put.x != -INFINITY) l = fmaf(put.y, ex2(put.x - m), l);
@@ -821,8 +825,8 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll 1
             for (int k = 0; k < HD / 32; k++) {
                 uint32_t o[32];
-                total(k, o, put);
                 __syncwarp();
+                total(k, o, put);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     float4 v;
