@@ -79,6 +79,20 @@ __device__ __forceinline__ uint16_t kq_e4m3x2(float lo, float hi) { // round to 
 __device__ __forceinline__ void kq_e4m3x4_h2(uint32_t w, uint32_t &lo, uint32_t &hi) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
+// two numbers as f16, and what that leaves of them
+__device__ __forceinline__ uint32_t kq_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t kq_h2_low(float a, float b, uint32_t hi) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    return kq_h2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ float kq_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // largest of a warp's values, none of them negative: their bits are in order
 __device__ __forceinline__ float kq_warp_top(float v) { return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v))); }
 // activations as f32

@@ -44,19 +44,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t h2_low(float a, float b, uint32_t hi) { // what hi = h2(a, b) leaves
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    return h2(a - f.x, b - f.y);
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 template <int HD, bool F8, int HT> struct Shape {
     static constexpr int R = 8 * HT, ES = F8 ? 1 : 2, ROW = HD * ES, NG = F8 ? 2 : 1, KT = 16 * NG; // groups of 16 positions of a warp's step
@@ -228,17 +215,17 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const float4 v = *reinterpret_cast<const float4 *>(&q_s[g + (HT == 2 ? 8 * h : 0)][d]);
-                        const uint32_t x = h2(v.x, v.y), y = h2(v.z, v.w);
+                        const uint32_t x = kq_h2(v.x, v.y), y = kq_h2(v.z, v.w);
                         if (HT == 2 || h == 0) {
                             qh[ks][h] = x;
                             qh[ks][h + 2] = y;
                             if (SPLIT && HT == 2) {
-                                ql[SPLIT && HT == 2 ? ks : 0][h] = h2_low(v.x, v.y, x);
-                                ql[SPLIT && HT == 2 ? ks : 0][h + 2] = h2_low(v.z, v.w, y);
+                                ql[SPLIT && HT == 2 ? ks : 0][h] = kq_h2_low(v.x, v.y, x);
+                                ql[SPLIT && HT == 2 ? ks : 0][h + 2] = kq_h2_low(v.z, v.w, y);
                             }
                         } else {
-                            qh[ks][h] = SPLIT ? h2_low(v.x, v.y, x) : 0u;
-                            qh[ks][h + 2] = SPLIT ? h2_low(v.z, v.w, y) : 0u;
+                            qh[ks][h] = SPLIT ? kq_h2_low(v.x, v.y, x) : 0u;
+                            qh[ks][h + 2] = SPLIT ? kq_h2_low(v.z, v.w, y) : 0u;
                         }
                     }
                 }
@@ -321,7 +308,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                         mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
                         const float mn = fmaxf(m[h], mx[h]), sub = mn == -INFINITY ? 0.f : mn - 14.f;
-                        alpha[h] = mn == -INFINITY ? 0.f : ex2(m[h] - mn); // nothing seen before: 2^-inf = 0
+                        alpha[h] = mn == -INFINITY ? 0.f : kq_ex2(m[h] - mn); // nothing seen before: 2^-inf = 0
                         same = same && m[h] == mn;
                         m[h] = mn;
                         float sum = 0.f;
@@ -329,10 +316,10 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                         for (int n = 0; n < NG; n++)
 #pragma unroll
                             for (int nt = 0; nt < 2; nt++) {
-                                const float p0 = ex2(sc[n][nt][2 * h] - sub), p1 = ex2(sc[n][nt][2 * h + 1] - sub); // up to 2^14: small ones keep their bits in f16
+                                const float p0 = kq_ex2(sc[n][nt][2 * h] - sub), p1 = kq_ex2(sc[n][nt][2 * h + 1] - sub); // up to 2^14: small ones keep their bits in f16
                                 sum += p0 + p1;
-                                ph[n][h][nt] = h2(p0, p1);
-                                if (SPLIT) pl[SPLIT ? n : 0][h][nt] = h2_low(p0, p1, ph[n][h][nt]);
+                                ph[n][h][nt] = kq_h2(p0, p1);
+                                if (SPLIT) pl[SPLIT ? n : 0][h][nt] = kq_h2_low(p0, p1, ph[n][h][nt]);
                             }
                         l[h] = l[h] * alpha[h] + sum;
                     }
@@ -441,7 +428,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
                     for (int k = 0; k < PER; k++) v[k] = 0.f;
 #pragma unroll
                     for (int w = 0; w < NW; w++) {
-                        const float f = ex2(m_s[w][r] - sub);
+                        const float f = kq_ex2(m_s[w][r] - sub);
                         ll += f * l_s[w][r];
 #pragma unroll
                         for (int k = 0; k < PER; k += 4) { // dimensions d0 + 16 k ..
@@ -455,7 +442,7 @@ __global__ void __launch_bounds__(NT, Shape<HD, F8, HT>::CTAS) pages_decode_kern
 #pragma unroll
                         for (int k = 0; k < PER; k += 4) {
                             if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out + 16 * k) = make_float4(v[k] * inv, v[k + 1] * inv, v[k + 2] * inv, v[k + 3] * inv);
-                            else if constexpr (SPLIT) *reinterpret_cast<uint2 *>(out + 16 * k) = make_uint2(h2(v[k] * inv, v[k + 1] * inv), h2(v[k + 2] * inv, v[k + 3] * inv));
+                            else if constexpr (SPLIT) *reinterpret_cast<uint2 *>(out + 16 * k) = make_uint2(kq_h2(v[k] * inv, v[k + 1] * inv), kq_h2(v[k + 2] * inv, v[k + 3] * inv));
                             else {
                                 const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v[k] * inv, v[k + 1] * inv), __floats2bfloat162_rn(v[k + 2] * inv, v[k + 3] * inv)};
                                 *reinterpret_cast<uint2 *>(out + 16 * k) = *reinterpret_cast<const uint2 *>(b);
@@ -508,13 +495,13 @@ template <int HD, int R> __global__ void __launch_bounds__(512) pages_combine_ke
         float mn = m;
 #pragma unroll
         for (int j = 0; j < 8; j++) mn = fmaxf(mn, ml[j].x);
-        const float sub = mn == -INFINITY ? 0.f : mn, f0 = ex2(m - sub);
+        const float sub = mn == -INFINITY ? 0.f : mn, f0 = kq_ex2(m - sub);
         l *= f0;
 #pragma unroll
         for (int u = 0; u < N; u++) o[u].x *= f0, o[u].y *= f0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float f = ex2(ml[j].x - sub);
+            const float f = kq_ex2(ml[j].x - sub);
             l += f * ml[j].y;
 #pragma unroll
             for (int u = 0; u < N; u++) o[u].x += f * v[j][u].x, o[u].y += f * v[j][u].y;
@@ -530,14 +517,14 @@ template <int HD, int R> __global__ void __launch_bounds__(512) pages_combine_ke
         float mn = m;
 #pragma unroll
         for (int w = 1; w < W; w++) mn = fmaxf(mn, ml_s[warp + w].x);
-        const float sub = mn == -INFINITY ? 0.f : mn, f0 = ex2(m - sub);
+        const float sub = mn == -INFINITY ? 0.f : mn, f0 = kq_ex2(m - sub);
         l *= f0;
 #pragma unroll
         for (int u = 0; u < N; u++) o[u].x *= f0, o[u].y *= f0;
 #pragma unroll
         for (int w = 1; w < W; w++) {
             const float2 ml = ml_s[warp + w];
-            const float f = ex2(ml.x - sub);
+            const float f = kq_ex2(ml.x - sub);
             l += f * ml.y;
 #pragma unroll
             for (int u = 0; u < N; u++) {

@@ -67,11 +67,6 @@ __device__ __forceinline__ float add_f16(float c, uint32_t h) { // c and the low
     asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(c) : "h"((uint16_t)h), "f"(c));
     return c;
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // pairs of f32 in one register pair
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
     uint64_t r;
@@ -100,7 +95,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) { // NaN if one
 }
 __device__ __forceinline__ uint64_t exp2_sfu(uint64_t x) {
     const float2 v = unpack2(x);
-    return pack2(ex2(v.x), ex2(v.y));
+    return pack2(kq_ex2(v.x), kq_ex2(v.y));
 }
 // 2^x = 2^n 2^f, n the nearest whole number (added into the exponent), |f| <= 1/2: the cubic of least largest relative error there,
 // 7.5e-5 (a seventh of half a step of f16).  Below 2^-126 it gives next to nothing, as it should; a NaN is seen to with the maximum.
@@ -115,14 +110,6 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
     p = fma2(p, f, pack2(0.99992806f, 0.99992806f));
     const float2 tt = unpack2(t), pp = unpack2(p);
     return pack2(__int_as_float(__float_as_int(pp.x) + (__float_as_int(tt.x) << 23)), __int_as_float(__float_as_int(pp.y) + (__float_as_int(tt.y) << 23)));
-}
-__device__ __forceinline__ uint32_t h2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t h2_low(float a, float b, uint32_t hi) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
-    return h2(a - f.x, b - f.y);
 }
 
 template <int HD, bool F8, int QS> struct Layout {
@@ -602,7 +589,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
 #pragma unroll
                         for (int p = 0; p < QS; p++) {
                             uint8_t *at = rows8 + p * (2 * L::TILE) + (d >> 6) * HALF + k * 128 + ((((d >> 3) & 7) ^ k) << 4) + (d & 7) * 2;
-                            const uint32_t hi = h2(v0, v1), v = p ? h2_low(v0, v1, hi) : hi;
+                            const uint32_t hi = kq_h2(v0, v1), v = p ? kq_h2_low(v0, v1, hi) : hi;
                             if (two) *reinterpret_cast<uint32_t *>(at) = v;
                             else *reinterpret_cast<uint16_t *>(at) = (uint16_t)v;
                         }
@@ -646,7 +633,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 tmem_ld32(to + 32 * k, o);
                 tmem_ld_wait();
                 if (put.x != -INFINITY) {
-                    const float f = ex2(put.x - m);
+                    const float f = kq_ex2(put.x - m);
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         const float4 v = *reinterpret_cast<const float4 *>(aside + (8 * k + j / 4) * (4 * R));
@@ -682,7 +669,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                         if (!*abort) tmem_st32(to + 32 * k, o);
                     }
                     tmem_st_wait();
-                    put.y = l + (put.x != -INFINITY ? put.y * ex2(put.x - m) : 0.f);
+                    put.y = l + (put.x != -INFINITY ? put.y * kq_ex2(put.x - m) : 0.f);
                     put.x = m;
                     l = 0.f;
                     joined = 0;
@@ -721,7 +708,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                 const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * crow;
                 const bool grown = !(top <= m + GROWTH) || m == -INFINITY; // the first tile, or a maximum that would make probabilities too large
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float mn = grown ? max3(m, top, top) : m, alpha = mn == m ? 1.f : ex2(m - mn);
+                    const float mn = grown ? max3(m, top, top) : m, alpha = mn == m ? 1.f : kq_ex2(m - mn);
                     m = mn;
                     if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                         l *= alpha;
@@ -760,7 +747,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                             v = BF && j % 8 < POLY ? exp2_poly(v) : exp2_sfu(v);
                             if (BF) sums[j & 1] = add2(sums[j & 1], v);
                             const float2 p = unpack2(v);
-                            hi[j] = h2(p.x, p.y);
+                            hi[j] = kq_h2(p.x, p.y);
                             // f16: the divisor is the sum of the weights as O has them, rounded, so that one weight's rounding is not the result's.  (Two parts
                             // as in f32 take 2048 rows at 6144 from 385 to 484 us, for results 1.01 instead of 1.13 half steps off.)
                             if (PS == 1 && !BF) {
@@ -769,7 +756,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                             }
                             if (PS == 2) {
                                 sums[j >> 3] = add2(sums[j >> 3], v);
-                                const uint32_t rest = h2_low(p.x, p.y, hi[j]);
+                                const uint32_t rest = kq_h2_low(p.x, p.y, hi[j]);
                                 if (e == 0) lo_even[PS == 2 ? j : 0] = rest;
                                 else lo[PS == 2 ? j : 0] = rest;
                             }
@@ -809,7 +796,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
             __syncwarp();
             after_sync();
             if (BF && w.take > FLUSH<T>) put = *put_at();
-            if (put.x != -INFINITY) l = fmaf(put.y, ex2(put.x - m), l);
+            if (put.x != -INFINITY) l = fmaf(put.y, kq_ex2(put.x - m), l);
             const bool whole = w.ub == 0 && w.take == w.n_units, ok = my_row_ok && !*abort;
             const float inv = m == -INFINITY ? 0.f : whole ? 1.f / l : 1.f; // a row that saw nothing is 0
             // 32 columns a time through the warp's part of the queries' room, so that a store writes whole lines of 4 rows
@@ -844,7 +831,7 @@ __global__ void __launch_bounds__(F8 ? 512 : 384, 1)
                     else {
                         T *out = (T *)a.out + to_row[j] + 32 * k;
                         if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(out) = v;
-                        else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<uint2 *>(out) = make_uint2(h2(v.x, v.y), h2(v.z, v.w));
+                        else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<uint2 *>(out) = make_uint2(kq_h2(v.x, v.y), kq_h2(v.z, v.w));
                         else {
                             const __nv_bfloat162 b[2] = {__floats2bfloat162_rn(v.x, v.y), __floats2bfloat162_rn(v.z, v.w)};
                             *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(b);
@@ -909,13 +896,13 @@ template <int HD> __global__ void __launch_bounds__(256) pages_join_kernel(const
             float mn = m[k];
 #pragma unroll
             for (int j = 0; j < 4; j++) mn = fmaxf(mn, k ? ml[j].z : ml[j].x);
-            const float sub = mn == -INFINITY ? 0.f : mn, f0 = ex2(m[k] - sub);
+            const float sub = mn == -INFINITY ? 0.f : mn, f0 = kq_ex2(m[k] - sub);
             l[k] *= f0;
 #pragma unroll
             for (int u = 0; u < N; u++) o[k][u].x *= f0, o[k][u].y *= f0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float f = ex2((k ? ml[j].z : ml[j].x) - sub);
+                const float f = kq_ex2((k ? ml[j].z : ml[j].x) - sub);
                 l[k] += f * (k ? ml[j].w : ml[j].y);
 #pragma unroll
                 for (int u = 0; u < N; u++) o[k][u].x += f * v[k][j][u].x, o[k][u].y += f * v[k][j][u].y;
